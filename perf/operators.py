@@ -174,8 +174,7 @@ def _plain_recurrence(s):
         E = dy * col(inside) + col(last) * dh[seq]
         back = back * col(~last)
     else:
-        E = dy
-        E[-1] += dh
+        E = torch.cat([dy[:-1], dy[-1:] + dh])
     G = _scan(back.flip(0), E.flip(0)).flip(0)
     if packed:
         prev = torch.cat([H[:1], H[:-1]])

@@ -687,6 +687,55 @@ int nsb_modulation_fwd(const void* raw_beta, const void* raw_alpha, const void* 
                        float v_th_min, int64_t rows, int64_t channels, void* beta, void* u,
                        void* v_th, void* omega, int dtype_in, int dtype_out, void* stream);
 
+/*
+ * Gated linear recurrence: the PLIF membrane without its spike (v = beta*v + (1-beta)*x,
+ * atomic_ops/plif_node.py:117-134), its gate per step from a raw projection. The reference
+ * has no counterpart (its linear recurrence takes finished coefficients,
+ * atomic_ops/parallel_scan.py:1282-1302).
+ *   f[t] = sigmoid(raw[t] + bias);  h[t] = f[t]*h[t-1] + (1-f[t])*x[t];  y[t] = h[t]
+ * State in fp32. raw, x: T rows of B x D values in `dtype`, element (t, b, d) at
+ * t*stride_t + b*stride_b + d (strides in elements: halves of one projection need no copy).
+ * y [T, B, D] contiguous; bias [D] or NULL; h0, h_last [B, D] fp32, h0 NULL = zeros.
+ *
+ * Packed sequences: B = 1 and cu_seqlens = seqs + 1 int32 in device memory; sequence s is
+ * rows cu_seqlens[s] .. cu_seqlens[s+1]-1, it starts from h0[s] and leaves h_last[s]
+ * ([seqs, D]). Lengths may be zero (h_last = h0). Rows outside of every sequence get y = 0.
+ * The values must not decrease; whatever they are, nothing outside the T rows and the
+ * `seqs` states is touched. cu_seqlens = NULL and seqs = 0: B sequences of T rows.
+ *
+ * ckpt: NULL, or nsb_gated_chunks(T) * B * D floats for the backward.
+ * scratch: nsb_gated_scratch_words(T, B*D) words that the call overwrites, 16-byte
+ * aligned; needed where that is not 0. One buffer per call in flight.
+ * Results do not depend on the order in which blocks run. Bounded waits inside, reported
+ * as those of the scan family are (bit 22 of the error word).
+ */
+int64_t nsb_gated_chunks(int64_t T);
+int64_t nsb_gated_scratch_words(int64_t T, int64_t cols);
+int nsb_gated_recurrence_fwd(const void* raw, int64_t raw_stride_t, int64_t raw_stride_b, const void* x,
+                             int64_t x_stride_t, int64_t x_stride_b, const float* bias, const float* h0,
+                             const int32_t* cu_seqlens, int64_t seqs, void* y, float* h_last, float* ckpt,
+                             uint32_t* scratch, int64_t T, int64_t B, int64_t D, int dtype, void* stream);
+
+/*
+ * Its gradient, with G[t] = dy[t] + f[t+1]*G[t+1] (+ dh_last at a sequence's last row):
+ *   d_x = (1-f)*G;  d_raw = G*(h[t-1]-x[t])*f*(1-f);  d_bias = sum d_raw;  d_h0 = f[0]*G[0]
+ * dy, d_raw, d_x [T, B, D] contiguous in `dtype`; d_bias [D], d_h0 and dh_last as h0, fp32.
+ * dh_last may be NULL (zeros), and so may each gradient that is not wanted. d_bias needs
+ * bias_part, nsb_gated_chunks(T) * B * D floats that the call overwrites, and is summed in
+ * a fixed order. Rows outside of every sequence get zero.
+ */
+int nsb_gated_recurrence_bwd(const void* raw, int64_t raw_stride_t, int64_t raw_stride_b, const void* x,
+                             int64_t x_stride_t, int64_t x_stride_b, const float* bias, const float* h0,
+                             const int32_t* cu_seqlens, int64_t seqs, const float* ckpt, const void* dy,
+                             const float* dh_last, void* d_raw, void* d_x, float* d_bias, float* d_h0,
+                             float* bias_part, uint32_t* scratch, int64_t T, int64_t B, int64_t D,
+                             int dtype, void* stream);
+
+/* One step for B rows, the state h [B, D] fp32 updated in place; y [B, D] contiguous. */
+int nsb_gated_recurrence_step(const void* raw, int64_t raw_stride_b, const void* x, int64_t x_stride_b,
+                              const float* bias, float* h, void* y, int64_t B, int64_t D, int dtype,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,6 +99,14 @@ _SIGNATURES = {
                                                             c_void_p]),
     "nsb_lateral_inhibition_bwd_static": (c_int, [c_void_p] * 5 + [c_int64, c_int64, c_float, c_int,
                                                                    c_int, c_void_p]),
+    "nsb_gated_chunks": (c_int64, [c_int64]),
+    "nsb_gated_scratch_words": (c_int64, [c_int64, c_int64]),
+    "nsb_gated_recurrence_fwd": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                         c_void_p, c_int64] + [c_void_p] * 4 + [c_int64] * 3 + [c_int, c_void_p]),
+    "nsb_gated_recurrence_bwd": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                         c_void_p, c_int64] + [c_void_p] * 9 + [c_int64] * 3 + [c_int, c_void_p]),
+    "nsb_gated_recurrence_step": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
+                                          c_int64, c_int, c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

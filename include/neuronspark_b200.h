@@ -736,6 +736,25 @@ int nsb_gated_recurrence_step(const void* raw, int64_t raw_stride_b, const void*
                               const float* bias, float* h, void* y, int64_t B, int64_t D, int dtype,
                               void* stream);
 
+/*
+ * A whole mixture-of-experts layer for a few tokens (serving; no gradient). The reference
+ * evaluates its experts one layer at a time for all tokens and merges their outputs
+ * (atomic_ops/moe_snn_ffn.py:164-261, atomic_ops/moe_kernels.py:210-224); for a few tokens
+ * this reads each routed expert's weights once and nothing of the others:
+ *   l = x Wr^T;  S = the K largest l of a token (ties: lowest index);  p = softmax of l over S
+ *   out = shared + sum over e in S of p_e * Wout_e ( silu(Wg_e x) * (Wu_e x) )
+ * x [N, D] with x_stride elements between rows; w_router [E, D]; w_in [E, 2F, D], rows
+ * 0..F-1 = Wg, F..2F-1 = Wu; w_out [E, D, F]; shared [N, D] or NULL; out [N, D]; all in
+ * `dtype`. ids [N, K] int32 and probs [N, K] fp32: each token's experts, best first, and p.
+ * N <= 64, K <= 16, K <= E <= 1024, D and F <= 2^20. Products accumulate in fp32; hidden
+ * values keep at least 16 significant bits between the two products.
+ * scratch: nsb_moe_few_tokens_scratch_bytes bytes, 16-byte aligned; one per call in flight.
+ */
+int64_t nsb_moe_few_tokens_scratch_bytes(int64_t N, int64_t E, int64_t K, int64_t D, int64_t F);
+int nsb_moe_few_tokens(const void* x, int64_t x_stride, const void* w_router, const void* w_in, const void* w_out,
+                       const void* shared, void* out, int32_t* ids, float* probs, void* scratch, int64_t N,
+                       int64_t E, int64_t K, int64_t D, int64_t F, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,6 +99,8 @@ _SIGNATURES = {
                                                             c_void_p]),
     "nsb_lateral_inhibition_bwd_static": (c_int, [c_void_p] * 5 + [c_int64, c_int64, c_float, c_int,
                                                                    c_int, c_void_p]),
+    "nsb_moe_few_tokens_scratch_bytes": (c_int64, [c_int64] * 5),
+    "nsb_moe_few_tokens": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + [c_int64] * 5 + [c_int, c_void_p]),
     "nsb_gated_chunks": (c_int64, [c_int64]),
     "nsb_gated_scratch_words": (c_int64, [c_int64, c_int64]),
     "nsb_gated_recurrence_fwd": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,

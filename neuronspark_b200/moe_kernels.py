@@ -1,6 +1,7 @@
 """Mixture-of-experts output combine (mirror of the reference's ``atomic_ops/moe_kernels.py``), and
 the same merge done on spike frames (``frames_combine``: what ``MoESNNFFN.forward_parallel`` computes
 with fp16_decode, a weighted sum and binary_encode_ste, ``atomic_ops/moe_snn_ffn.py:377-393``).
+``moe_few_tokens`` is a whole layer of continuous experts for the few tokens of a decoding step.
 
     out[n, d] = shared[n, d] + sum_e experts[e, n, d] * weights[n, e]
 
@@ -110,3 +111,54 @@ def frames_combine(shared: torch.Tensor, experts: torch.Tensor, weights: torch.T
     """Reference: atomic_ops/moe_snn_ffn.py:377-393 (the training branch's decode / combine / add
     residual / binary_encode_ste sequence)."""
     return FramesCombine.apply(shared, experts, weights, residual)
+
+
+#: Most tokens of one ``moe_few_tokens`` call.
+MOE_FEW_TOKENS_MAX = 64
+
+
+def moe_few_tokens(x: torch.Tensor, w_router: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, top_k: int,
+                   shared: torch.Tensor | None = None, return_routing: bool = False):
+    """A whole mixture-of-experts layer for the few tokens (at most 64) of a decoding step: routing, the chosen
+    experts' gated products and the weighted sum, reading every chosen expert's weights once.
+
+        l = x @ w_router.T;  the ``top_k`` largest of a token are taken (ties: lowest index), p = their softmax
+        out = shared + sum_e p_e * (silu(w_in[e, :F] @ x) * (w_in[e, F:] @ x)) @ w_out[e].T
+
+    ``x`` [N, D] (rows may be strided), ``w_router`` [E, D], ``w_in`` [E, 2F, D], ``w_out`` [E, D, F], ``shared``
+    [N, D] or None, all of one type (float32, bfloat16 or float16). ``top_k`` <= 16, E <= 1024. Returns ``out``
+    [N, D], and with ``return_routing`` also the experts' numbers [N, top_k] (int32, best first) and p (float32).
+    For serving: no gradients. ``moe_combine`` merges outputs of experts that were all evaluated."""
+    if x.dim() != 2 or w_router.dim() != 2 or w_in.dim() != 3 or w_out.dim() != 3:
+        raise NSBError("moe_few_tokens expects x (N, D), w_router (E, D), w_in (E, 2F, D), w_out (E, D, F)")
+    (N, D), E, F = x.shape, w_router.shape[0], w_out.shape[2]
+    if (w_router.shape != (E, D) or w_in.shape != (E, 2 * F, D) or w_out.shape != (E, D, F)
+            or (shared is not None and shared.shape != x.shape)):
+        raise NSBError("moe_few_tokens: inconsistent shapes")
+    if not 1 <= top_k <= min(E, 16) or E > 1024 or N > MOE_FEW_TOKENS_MAX:
+        raise NSBError(f"moe_few_tokens takes up to {MOE_FEW_TOKENS_MAX} tokens, up to 1024 experts and 1 to min(E, 16) "
+                       f"experts per token, got N={N}, E={E}, top_k={top_k}")
+    tensors = [x, w_router, w_in, w_out] + ([shared] if shared is not None else [])
+    code = _lib.dtype_code(x.dtype)
+    if any(t.dtype != x.dtype for t in tensors):
+        raise NSBError("moe_few_tokens: all tensors have one type")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise NSBError("moe_few_tokens has no gradients; call it under torch.no_grad()")
+    if not (w_router.is_contiguous() and w_in.is_contiguous() and w_out.is_contiguous()):
+        raise NSBError("moe_few_tokens: weights are laid out once, contiguously; none of them is copied here")
+    dev = _lib.require_cuda(*tensors)
+    if D > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    if shared is not None:
+        shared = shared.contiguous()
+    L = _lib.lib()
+    out = torch.empty((N, D), dtype=x.dtype, device=dev)
+    ids = torch.empty((N, top_k), dtype=torch.int32, device=dev)
+    probs = torch.empty((N, top_k), dtype=torch.float32, device=dev)
+    scratch = torch.empty(int(L.nsb_moe_few_tokens_scratch_bytes(N, E, top_k, D, F)), dtype=torch.uint8, device=dev)
+    p = _lib.ptr
+    with torch.cuda.device(dev):
+        _lib.check(L.nsb_moe_few_tokens(p(x), x.stride(0), p(w_router), p(w_in), p(w_out), p(shared), p(out), p(ids),
+                                        p(probs), p(scratch), N, E, top_k, D, F, code, _lib.stream_ptr(dev)),
+                   "nsb_moe_few_tokens")
+    return (out, ids, probs) if return_routing else out

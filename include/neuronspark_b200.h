@@ -65,6 +65,10 @@ extern "C" {
                               this one is checked against torch autograd
                               through that primitive                           */
 
+/* ---- activations after a normalisation ---- */
+#define NSB_ACT_NONE 0
+#define NSB_ACT_SILU 1 /* z * sigmoid(z) */
+
 /* Library version (major*10000 + minor*100 + patch). */
 int nsb_version(void);
 
@@ -754,6 +758,29 @@ int64_t nsb_moe_few_tokens_scratch_bytes(int64_t N, int64_t E, int64_t K, int64_
 int nsb_moe_few_tokens(const void* x, int64_t x_stride, const void* w_router, const void* w_in, const void* w_out,
                        const void* shared, void* out, int32_t* ids, float* probs, void* scratch, int64_t N,
                        int64_t E, int64_t K, int64_t D, int64_t F, int dtype, void* stream);
+
+/*
+ * Group norm with an activation, channels last. x, y [N, L, C] contiguous in `dtype`; the
+ * statistics of a sample and a group of C/G channels go over all L positions (L = 1: the
+ * groups of a row each for themselves, as the heads of a token):
+ *   xh = (x - mean) * rsqrt(var + eps);  z = weight*xh + bias;  y = act(z)
+ * weight, bias [C] fp32 or NULL (ones, zeros). mean, rstd [N, G] fp32: both or neither,
+ * written for the backward. Variance (over n, not n - 1) about the mean, fp32 sums.
+ * scratch: nsb_group_norm_scratch_floats floats, needed where that is not 0; one buffer per
+ * call in flight. The reference has no counterpart; its normaliser takes whole rows and
+ * subtracts no mean (atomic_ops/lateral_inhibition.py:50-119).
+ */
+int64_t nsb_group_norm_scratch_floats(int64_t N, int64_t L, int64_t C, int64_t G, int backward);
+int nsb_group_norm_fwd(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
+                       float* scratch, int64_t N, int64_t L, int64_t C, int64_t G, float eps, int activation,
+                       int dtype, void* stream);
+
+/* Gradients, with d = dy*act'(z) and g = d*weight:
+ *   dx = rstd*(g - mean(g) - xh*mean(g*xh));  dweight = sum d*xh;  dbias = sum d
+ * Any of the three may be NULL. The sums over N and L are added in a fixed order. */
+int nsb_group_norm_bwd(const void* dy, const void* x, const float* weight, const float* bias, const float* mean,
+                       const float* rstd, void* dx, float* dweight, float* dbias, float* scratch, int64_t N,
+                       int64_t L, int64_t C, int64_t G, int activation, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -19,6 +19,7 @@ NSB_OK = 0
 F32, BF16, F16 = 0, 1, 2
 SURR_SIGMOID, SURR_ATAN = 0, 1
 RESIDUAL_EAGER, RESIDUAL_COMPILED = 0, 1
+ACT_NONE, ACT_SILU = 0, 1
 
 _DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
@@ -101,6 +102,9 @@ _SIGNATURES = {
                                                                    c_int, c_void_p]),
     "nsb_moe_few_tokens_scratch_bytes": (c_int64, [c_int64] * 5),
     "nsb_moe_few_tokens": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + [c_int64] * 5 + [c_int, c_void_p]),
+    "nsb_group_norm_scratch_floats": (c_int64, [c_int64] * 4 + [c_int]),
+    "nsb_group_norm_fwd": (c_int, [c_void_p] * 7 + [c_int64] * 4 + [c_float, c_int, c_int, c_void_p]),
+    "nsb_group_norm_bwd": (c_int, [c_void_p] * 10 + [c_int64] * 4 + [c_int, c_int, c_void_p]),
     "nsb_gated_chunks": (c_int64, [c_int64]),
     "nsb_gated_scratch_words": (c_int64, [c_int64, c_int64]),
     "nsb_gated_recurrence_fwd": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,

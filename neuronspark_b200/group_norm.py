@@ -1,0 +1,100 @@
+"""Group norm with an activation, channels last.
+
+    xh = (x - mean) / sqrt(var + eps)      z = weight * xh + bias      y = z * sigmoid(z)   (or y = z)
+
+The statistics of a sample and a group of C / num_groups channels go over all positions of the sample: ``x`` is
+[N, ..., C]. An [N, C] tensor has one position per sample, so every row's groups are normalised by themselves:
+what the heads of a recurrence's output want, token by token (reshape a time-major [T, B, D] to [T*B, D]).
+
+Beside ``lateral_inhibition.LateralInhibition`` / ``RMSNorm``, which normalise whole rows by their mean square;
+the reference has no group norm. CUDA tensors only; statistics and sums are fp32 whatever the type of ``x``.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from ._lib import NSBError
+
+_ACTIVATIONS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU}
+
+
+def _param(t):
+    return None if t is None else t.detach().to(torch.float32).contiguous()
+
+
+class GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, num_groups, eps, act):
+        x_c, w, b = x.detach().contiguous(), _param(weight), _param(bias)
+        dev = _lib.require_cuda(x_c, w, b)
+        N, C = x.shape[0], x.shape[-1]
+        L = x.numel() // (N * C) if N * C else 0
+        lib, code, p = _lib.lib(), _lib.dtype_code(x.dtype), _lib.ptr
+        y = torch.empty_like(x_c)
+        needs_grad = any(ctx.needs_input_grad)
+        stats = torch.empty((2, N, num_groups), dtype=torch.float32, device=dev) if needs_grad else (None, None)
+        words = int(lib.nsb_group_norm_scratch_floats(N, L, C, num_groups, 0))
+        scratch = torch.empty(words, dtype=torch.float32, device=dev) if words else None
+        with torch.cuda.device(dev):
+            _lib.check(lib.nsb_group_norm_fwd(p(x_c), p(w), p(b), p(y), p(stats[0]), p(stats[1]), p(scratch), N, L, C,
+                                              num_groups, eps, act, code, _lib.stream_ptr(dev)), "nsb_group_norm_fwd")
+        if needs_grad:
+            ctx.save_for_backward(x_c, w, b, stats)
+            ctx.sizes = (N, L, C, num_groups, act)
+            ctx.in_dtypes = tuple(t.dtype if t is not None else None for t in (weight, bias))
+        return y
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        x, w, b, stats = ctx.saved_tensors
+        N, L, C, G, act = ctx.sizes
+        dev, lib, p = x.device, _lib.lib(), _lib.ptr
+        dy = _lib.convert(grad_out, x.dtype)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty(C, dtype=torch.float32, device=dev) if need_w and w is not None else None
+        db = torch.empty(C, dtype=torch.float32, device=dev) if need_b and b is not None else None
+        words = int(lib.nsb_group_norm_scratch_floats(N, L, C, G, 1))
+        scratch = torch.empty(words, dtype=torch.float32, device=dev) if words else None
+        with torch.cuda.device(dev):
+            _lib.check(lib.nsb_group_norm_bwd(p(dy), p(x), p(w), p(b), p(stats[0]), p(stats[1]), p(dx), p(dw), p(db),
+                                              p(scratch), N, L, C, G, act, _lib.dtype_code(x.dtype), _lib.stream_ptr(dev)),
+                       "nsb_group_norm_bwd")
+        dw, db = (None if g is None else g.to(t) for g, t in zip((dw, db), ctx.in_dtypes))
+        return dx, dw, db, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                   eps: float = 1e-5, activation: str | None = "silu") -> torch.Tensor:
+    """``x`` [N, ..., C] (float32, bfloat16 or float16), ``weight`` and ``bias`` [C] or None. ``activation`` is
+    "silu" or None. Returns a contiguous tensor of ``x``'s shape and type; gradients for x, weight and bias."""
+    if x.dim() < 2:
+        raise NSBError("group_norm_act expects x of [N, ..., C]")
+    C = x.shape[-1]
+    if num_groups < 1 or C % num_groups:
+        raise NSBError(f"group_norm_act: {C} channels do not divide into {num_groups} groups")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and tuple(t.shape) != (C,):
+            raise NSBError(f"{name} has shape {tuple(t.shape)}, expected {(C,)}")
+    if activation not in _ACTIVATIONS:
+        raise NSBError(f"unknown activation {activation!r}; expected 'silu' or None")
+    _lib.dtype_code(x.dtype)
+    return GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps), _ACTIVATIONS[activation])
+
+
+class GroupNorm(nn.Module):
+    """``group_norm_act`` with its parameters, channels last."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, activation: str | None = "silu"):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(num_channels))
+        self.bias = nn.Parameter(torch.zeros(num_channels))
+        self.num_groups, self.eps, self.activation = num_groups, eps, activation
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+
+    def extra_repr(self):
+        return f"{self.num_groups}, {self.weight.numel()}, eps={self.eps}, activation={self.activation}"

@@ -7,8 +7,8 @@
 //   G_t = dy_t + K_{t+1}     dx_t = (1 - f_t) G_t     draw_t = G_t (h_{t-1} - x_t) f_t (1 - f_t)
 //
 // Each step is an affine map of the state, h -> P h + H, and such maps compose associatively, so time is
-// cut into chunks that are worked on side by side. A CTA takes one chunk of one block of columns: every
-// warp holds S steps of 32 V columns in registers, finds their composed map, the CTA's warps exchange
+// cut into chunks that are worked on side by side. A tile is one chunk (at most 64 steps) of one block of columns:
+// every warp has S steps of 32 V columns in registers, finds their composed map, the CTA's warps exchange
 // their maps through shared memory, CTAs exchange theirs through global memory (below), and every warp then
 // runs its steps once more from its true starting state. Each input is read once and each output written
 // once; the only other traffic is 4-12 bytes per chunk and column.
@@ -18,9 +18,14 @@
 // state after the group before, taken through the maps of the chunks of its own group that precede it, always
 // in the same order: results do not depend on timing. A published word is its own flag: the scratch is
 // filled with 0xff bytes, which no published value has (see publishable), and 8-byte words are written
-// whole. Work is handed out by a ticket counter in order of time, so whatever a CTA waits for belongs to a
-// CTA that is running or has finished; every wait is bounded all the same and hands on NaN if it gives up.
+// whole. Tiles are handed out by a ticket counter in order of time and a CTA works on its tickets in order, so
+// whatever a tile waits for is being worked on or finished; every wait is bounded all the same and hands on NaN
+// if it gives up.
+//
+// CTAs stay and take tile after tile: the next tile's inputs are copied to shared memory (by the thread that
+// will use them, so that nothing needs a barrier) while this one is worked on.
 #include <algorithm>
+#include <atomic>
 
 #include "nsb_common.cuh"
 
@@ -29,6 +34,8 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
+constexpr int kFwdSteps = 16, kBwdSteps = 8;  // steps of a warp's tile
+constexpr int kCkptRows = 64;                 // rows between the states that the forward saves: a backward chunk
 constexpr uint32_t kEmpty = 0xffffffffu;
 constexpr uint32_t kErrGated = 0x00400000u;
 
@@ -39,9 +46,8 @@ struct GatedParams {
   void *y, *d_raw, *d_x;
   float *h_last, *ckpt, *d_h0, *d_bias_part;
   long long raw_st, raw_sb, x_st, x_sb;  // strides in elements between rows and between blocks of Dw columns
-  long long T, cols, Dw, D;         // D: period of the bias
-  long long nb;                     // column blocks
-  int nchunks, g, wt, S_seqs;
+  int T, cols, Dw, D;               // D: period of the bias
+  int nb, nchunks, g, wt, S_seqs;   // nb: column blocks
   uint32_t* ticket;
   uint2* maps;                      // [nchunks][cols] (P, H)
   uint32_t* states;                 // [nchunks / g][cols]
@@ -49,27 +55,78 @@ struct GatedParams {
   unsigned long long limit_ns;
 };
 
-// sigmoid(a) and sigmoid(-a), both to a few units in the last place of fp32 over the whole range: the
-// exponential is taken of -|a|, so it neither overflows nor is subtracted from one.
-__device__ __forceinline__ void gate(float a, float& f, float& m) {
-  const float t = __expf(-fabsf(a));
-  const float big = __fdividef(1.0f, 1.0f + t), small = t * big;
-  f = a >= 0.0f ? big : small;
-  m = a >= 0.0f ? small : big;
+// Arithmetic on a thread's V columns, two per instruction where V allows (same roundings).
+#define NSB_PAIR(x, i) (*reinterpret_cast<unsigned long long*>(&(x)[i]))
+#define NSB_CPAIR(x, i) (*reinterpret_cast<const unsigned long long*>(&(x)[i]))
+template <int V>
+struct alignas(V >= 2 ? 8 : 4) Cols {
+  float v[V];
+  __device__ __forceinline__ float& operator[](int i) { return v[i]; }
+  __device__ __forceinline__ const float& operator[](int i) const { return v[i]; }
+};
+template <int V>
+__device__ __forceinline__ Cols<V> all(float c) {
+  Cols<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r[i] = c;
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Cols<V> fma(const Cols<V>& a, const Cols<V>& b, const Cols<V>& c) {
+  Cols<V> r;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(NSB_PAIR(r.v, i))
+          : "l"(NSB_CPAIR(a.v, i)), "l"(NSB_CPAIR(b.v, i)), "l"(NSB_CPAIR(c.v, i)));
+  } else {
+    r[0] = fmaf(a[0], b[0], c[0]);
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Cols<V> mul(const Cols<V>& a, const Cols<V>& b) {
+  Cols<V> r;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(NSB_PAIR(r.v, i)) : "l"(NSB_CPAIR(a.v, i)), "l"(NSB_CPAIR(b.v, i)));
+  } else {
+    r[0] = __fmul_rn(a[0], b[0]);
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Cols<V> add(const Cols<V>& a, const Cols<V>& b) {
+  Cols<V> r;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      asm("add.rn.f32x2 %0, %1, %2;" : "=l"(NSB_PAIR(r.v, i)) : "l"(NSB_CPAIR(a.v, i)), "l"(NSB_CPAIR(b.v, i)));
+  } else {
+    r[0] = __fadd_rn(a[0], b[0]);
+  }
+  return r;
 }
 
-// The pair in one register: the smaller of f and 1 - f, negative where that is f. The other is one minus it,
-// which costs neither any digits.
-__device__ __forceinline__ float gate_packed(float a) {
-  const float t = __expf(-fabsf(a));
-  return copysignf(t * __fdividef(1.0f, 1.0f + t), a);
+// f = sigmoid(a + b) and m = sigmoid(-(a + b)) from e = exp(-(a + b)): f = 1 / (1 + e), m = e f, neither of them
+// a difference, so both keep their digits however small they are. The exponent is capped where f is 2^-126
+// (e f must not become inf * 0); min.NaN lets a NaN through. `b2` = -b log2(e).
+constexpr float kLog2e = 1.4426950408889634f;
+template <int V>
+__device__ __forceinline__ void gate(const Cols<V>& a, const Cols<V>& b2, Cols<V>& f, Cols<V>& m) {
+  Cols<V> q = fma<V>(a, all<V>(-kLog2e), b2), e;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(q[v]) : "f"(q[v]));  // 126
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[v]) : "f"(q[v]));
+  }
+  q = add<V>(e, all<V>(1.0f));
+#pragma unroll
+  for (int v = 0; v < V; ++v) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f[v]) : "f"(q[v]));
+  m = mul<V>(e, f);
 }
-__device__ __forceinline__ void gate_unpack(float g, float& f, float& m) {
-  const float small = fabsf(g), big = 1.0f - small;
-  const bool shut = __float_as_int(g) < 0;
-  f = shut ? small : big;
-  m = shut ? big : small;
-}
+__device__ __forceinline__ float gate_bias(float b) { return b * -kLog2e; }
 
 __device__ __forceinline__ uint32_t publishable(float v) {
   const uint32_t b = __float_as_uint(v);
@@ -80,11 +137,12 @@ __device__ __forceinline__ uint32_t peek32(const uint32_t* p) {
   asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ uint2 peek64(const uint2* p) {
+__device__ __forceinline__ unsigned long long peek64(const uint2* p) {
   unsigned long long v;
   asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-  return make_uint2((uint32_t)v, (uint32_t)(v >> 32));
+  return v;
 }
+__device__ __forceinline__ float published(uint32_t w) { return __uint_as_float(w == kEmpty ? 0x7fffffffu : w); }
 __device__ __forceinline__ void post32(uint32_t* p, uint32_t v) {
   asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
@@ -93,29 +151,18 @@ __device__ __forceinline__ void post64(uint2* p, uint32_t a, uint32_t b) {
                : "memory");
 }
 
-// Bounded wait for a published word; NaN if it gives up (and the error word says so).
-template <typename Peek, typename Full>
-__device__ __forceinline__ auto await_word(Peek peek, Full full, const GatedParams& p) {
-  auto v = peek();
-  if (full(v)) return v;
+// Bounded waits for published words: `look` reads them again, all at once, until it finds them all there. Words that
+// never came read as NaN (and the error word says so).
+template <typename Look>
+__device__ __forceinline__ void await(Look look, const GatedParams& p) {
+  if (look()) return;
   const uint64_t t0 = global_timer_ns();
   uint32_t it = 0;
-  while (!full(v = peek())) {
+  while (!look())
     if ((++it & 0x3F) == 0 && (global_timer_ns() - t0 > p.limit_ns || it > (1u << 28))) {
       if (p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), kErrGated);
-      break;
+      return;
     }
-  }
-  return v;
-}
-__device__ __forceinline__ float await_state(const uint32_t* w, const GatedParams& p) {
-  const uint32_t v = await_word([&] { return peek32(w); }, [](uint32_t b) { return b != kEmpty; }, p);
-  return __uint_as_float(v == kEmpty ? 0x7fffffffu : v);
-}
-__device__ __forceinline__ float2 await_map(const uint2* w, const GatedParams& p) {
-  uint2 v = await_word([&] { return peek64(w); }, [](uint2 b) { return b.x != kEmpty; }, p);
-  if (v.x == kEmpty) v = make_uint2(0x7fffffffu, 0x7fffffffu);
-  return make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
 }
 
 // What the S rows of a warp are: bit s of `in` - row s belongs to a sequence; `first`, `last` - it is that
@@ -123,426 +170,608 @@ __device__ __forceinline__ float2 await_map(const uint2* w, const GatedParams& p
 struct Rows {
   uint32_t in, first, last;
   int seq;
+  // nothing but rows in the middle of a sequence
+  __device__ __forceinline__ bool plain(int S) const { return in == (1u << S) - 1u && !(first | last); }
 };
 template <int S, bool PACKED>
-__device__ __forceinline__ Rows row_kinds(const GatedParams& p, long long t0, int lane) {
+__device__ __forceinline__ Rows row_kinds(const GatedParams& p, int t0, int lane) {
   Rows r;
-  const long long t = t0 + lane;
-  bool in = lane < S && t < p.T, first = false, last = false;
   r.seq = 0;
   if constexpr (PACKED) {
-    if (in) {
-      int lo = 0, hi = p.S_seqs;  // sequences that end at or before row t
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(p.cu + mid + 1) <= t) lo = mid + 1; else hi = mid;
+    // 32 guesses at a time: lo = number of sequences that end at or before row t0
+    int lo = 0, n = p.S_seqs;  // it lies in lo .. lo + n
+    while (n > 0) {
+      const int step = (n + 31) / 32, at = lane * step;
+      const uint32_t b = __ballot_sync(0xffffffffu, at < n && __ldg(p.cu + lo + at + 1) <= t0);
+      const int k = __popc(b);  // guesses 0 .. k - 1 hold, guess k does not
+      if (k == 0) break;
+      lo += (k - 1) * step + 1;
+      n = min(step - 1, n - (k - 1) * step - 1);
+    }
+    // the ends around there, one per lane; each row counts those it has passed
+    const int w = lo + lane <= p.S_seqs ? __ldg(p.cu + lo + lane) : 0x7fffffff;
+    bool in = false, first = false, last = false;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int t = t0 + s;
+      const uint32_t passed = __ballot_sync(0xffffffffu, lane > 0 && w <= t);
+      int q = lo + __popc(passed), begin, end;
+      if (passed == 0xfffffffeu) {  // over 30 sequences, nearly all of them empty, end among these rows
+        int hi = p.S_seqs;
+        while (q < hi) {
+          const int mid = (q + hi) >> 1;
+          if (__ldg(p.cu + mid + 1) <= t) q = mid + 1; else hi = mid;
+        }
+        begin = q < p.S_seqs ? __ldg(p.cu + q) : 0;
+        end = q < p.S_seqs ? __ldg(p.cu + q + 1) : 0;
+      } else {
+        begin = __shfl_sync(0xffffffffu, w, q - lo);
+        end = __shfl_sync(0xffffffffu, w, q - lo + 1);
       }
-      in = lo < p.S_seqs && __ldg(p.cu + lo) <= t;
-      if (in) {
-        r.seq = lo;
-        first = __ldg(p.cu + lo) == t;
-        last = __ldg(p.cu + lo + 1) == t + 1;
+      if (lane == s) {
+        in = t < p.T && q < p.S_seqs && begin <= t;
+        r.seq = in ? q : 0;
+        first = in && begin == t;
+        last = in && end == t + 1;
       }
     }
+    r.in = __ballot_sync(0xffffffffu, in);
+    r.first = __ballot_sync(0xffffffffu, first);
+    r.last = __ballot_sync(0xffffffffu, last);
   } else {
-    first = in && t == 0;
-    last = in && t == p.T - 1;
+    const int left = p.T - t0;
+    r.in = left >= S ? (1u << S) - 1u : left > 0 ? (1u << left) - 1u : 0u;
+    r.first = t0 == 0 ? 1u : 0u;
+    r.last = left > 0 && left <= S ? 1u << (left - 1) : 0u;
   }
-  r.in = __ballot_sync(0xffffffffu, in);
-  r.first = __ballot_sync(0xffffffffu, first);
-  r.last = __ballot_sync(0xffffffffu, last);
   return r;
 }
 
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
-  return *reinterpret_cast<const Vec<T, V>*>(p);
-}
-
-// The map h -> P h + H of one step or of several. Where a sequence begins, the state from before must not come
-// in, not even as 0 * NaN: such a map has P = -0 (a product of gates is never negative) and gives H.
+// The map h -> P h + H of one step or of several. Where a sequence of a packed batch begins, the state from before
+// must not come in, not even as 0 * NaN: such a map has P = -0 (a product of gates is never negative) and gives H.
 template <int V>
 struct MapV {
-  float P[V], H[V];
+  Cols<V> P, H;
 };
 constexpr float kCut = -0.0f;
 __device__ __forceinline__ bool is_cut(float P) { return __float_as_uint(P) == 0x80000000u; }
-__device__ __forceinline__ float apply_map(float P, float H, float h) { return is_cut(P) ? H : fmaf(P, h, H); }
-// (P, H) followed by (P2, H2)
-__device__ __forceinline__ void then_map(float& P, float& H, float P2, float H2) {
-  H = apply_map(P2, H2, H);
-  P = is_cut(P2) || is_cut(P) ? kCut : P * P2;
+template <bool PACKED, int V>
+__device__ __forceinline__ Cols<V> apply_map(const Cols<V>& P, const Cols<V>& H, const Cols<V>& h) {
+  Cols<V> r = fma<V>(P, h, H);
+  if constexpr (PACKED)
+#pragma unroll
+    for (int v = 0; v < V; ++v) r[v] = is_cut(P[v]) ? H[v] : r[v];
+  return r;
+}
+// m, then (P, H)
+template <bool PACKED, int V>
+__device__ __forceinline__ void then_map(MapV<V>& m, const Cols<V>& P, const Cols<V>& H) {
+  m.H = apply_map<PACKED, V>(P, H, m.H);
+  Cols<V> r = mul<V>(m.P, P);
+  if constexpr (PACKED)
+#pragma unroll
+    for (int v = 0; v < V; ++v) r[v] = is_cut(m.P[v]) || is_cut(P[v]) ? kCut : r[v];
+  m.P = r;
 }
 
 // The state (or, in reverse, the hand-back) that a chunk starts from. `pos` counts chunks in the order in
-// which they are worked on. Every time warp takes the maps of some of the preceding chunks of the group and
-// composes them in order; the parts meet in shared memory. Returns the same value in every time warp.
+// which they are worked on. The state before the group was looked for when the tile was begun (`early`). With g = 1
+// that is all; otherwise every time warp takes the maps of four of the preceding chunks of the group and composes
+// them in order, and the parts meet in shared memory. Same value in every time warp.
 template <int V>
-__device__ __forceinline__ void chunk_start(const GatedParams& p, int pos, long long col, bool on, int wt_idx, int wt,
-                                            MapV<V>* part, int lane_slot, float (&start)[V]) {
-  const int group = pos / p.g, j = pos - group * p.g;
-  const int per = (j + wt - 1) / wt;
-  MapV<V> m;
+struct Early {
+  uint32_t w[V];
+  __device__ __forceinline__ void look(const GatedParams& p, int row, int col, bool on) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) m.P[v] = 1.0f, m.H[v] = 0.0f;
-  if (on) {
-    const int a = wt_idx * per, b = min(j, a + per);
-    const uint2* w = p.maps + (long long)(group * p.g + a) * p.cols + col;
-    for (int i = a; i < b; ++i, w += p.cols)
+    for (int v = 0; v < V; ++v) w[v] = 0;
+    if (row >= 0 && on)
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float2 q = await_map(w + v, p);
-        then_map(m.P[v], m.H[v], q.x, q.y);
-      }
-    if (wt_idx == 0) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float s = group ? await_state(p.states + (long long)(group - 1) * p.cols + col + v, p) : 0.0f;
-        m.H[v] = apply_map(m.P[v], m.H[v], s);
-      }
-    }
+      for (int v = 0; v < V; ++v) w[v] = peek32(p.states + (long long)row * p.cols + col + v);
   }
-  part[lane_slot] = m;
+  __device__ __forceinline__ bool there() const {
+    bool r = true;
+#pragma unroll
+    for (int v = 0; v < V; ++v) r = r && w[v] != kEmpty;
+    return r;
+  }
+};
+template <int V>
+__device__ __forceinline__ Cols<V> state_before(const GatedParams& p, Early<V>& early, int row, int col, bool on) {
+  if (!early.there()) await([&] { early.look(p, row, col, on); return early.there(); }, p);
+  Cols<V> r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) r[v] = published(early.w[v]);
+  return r;
+}
+// `part`: shared memory that nobody else uses from here to the caller's next barrier
+template <bool PACKED, int V>
+__device__ __forceinline__ Cols<V> chunk_start(const GatedParams& p, Early<V>& early, int pos, int col, bool on,
+                                               int wt_idx, int wt, MapV<V>* part, int first_slot) {
+  const int group = pos / p.g;
+  if (p.g == 1) return state_before<V>(p, early, group - 1, col, on);
+  const int j = pos - group * p.g;
+  constexpr int kMost = 4;  // 31 maps among 8 warps; with fewer time warps there is one chunk
+  MapV<V> m = {all<V>(1.0f), all<V>(0.0f)};
+  const int n = min(kMost, j - wt_idx * kMost);
+  if (on && n > 0) {
+    const uint2* w = p.maps + (long long)(group * p.g + wt_idx * kMost) * p.cols + col;
+    unsigned long long q[kMost][V];
+    await([&] {
+#pragma unroll
+      for (int i = 0; i < kMost; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) q[i][v] = i < n ? peek64(w + (long long)i * p.cols + v) : 0ull;
+      bool there = true;
+#pragma unroll
+      for (int i = 0; i < kMost; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) there = there && (uint32_t)q[i][v] != kEmpty;
+      return there;
+    }, p);
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+      if (i < n) {
+        Cols<V> P, H;
+#pragma unroll
+        for (int v = 0; v < V; ++v) P[v] = published((uint32_t)q[i][v]), H[v] = published((uint32_t)(q[i][v] >> 32));
+        then_map<PACKED, V>(m, P, H);
+      }
+  }
+  if (wt_idx == 0) m.H = apply_map<PACKED, V>(m.P, m.H, state_before<V>(p, early, group - 1, col, on));
+  part[threadIdx.x] = m;
   __syncthreads();
-#pragma unroll
-  for (int v = 0; v < V; ++v) start[v] = 0.0f;
-  const int stride = 32;
-  for (int i = 0; i < wt; ++i) {
-    const MapV<V> q = part[(lane_slot % stride) + i * stride + (lane_slot / (wt * stride)) * (wt * stride)];
-#pragma unroll
-    for (int v = 0; v < V; ++v) start[v] = i == 0 ? q.H[v] : apply_map(q.P[v], q.H[v], start[v]);
-  }
+  Cols<V> start = part[first_slot].H;
+  for (int i = 1; i < wt; ++i) start = apply_map<PACKED, V>(part[first_slot + i * 32].P, part[first_slot + i * 32].H, start);
+  return start;
 }
 
-template <typename T, int V, int S, bool PACKED, bool CHAIN>
-__global__ void __launch_bounds__(kThreads) gated_fwd_kernel(const GatedParams p) {
-  __shared__ MapV<V> maps[kThreads], part[CHAIN ? kThreads : 1];
-  __shared__ uint32_t s_ticket;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int wt = p.wt, wt_idx = warp % wt, wc_idx = warp / wt, wc = kWarps / wt;
-  long long work = blockIdx.x;
-  if constexpr (CHAIN) {
-    if (threadIdx.x == 0) s_ticket = atomicAdd(p.ticket, 1u) + 1u;  // (the counter starts at 0xffffffff)
-    __syncthreads();
-    work = s_ticket;
-  }
-  const int chunk = (int)(work / p.nb);
-  const long long col = ((work % p.nb) * wc + wc_idx) * (32 * V) + (long long)lane * V;
-  const bool on = col < p.cols;
-  const long long t0 = ((long long)chunk * wt + wt_idx) * S;
-  const T* raw = static_cast<const T*>(p.raw);
-  const T* x = static_cast<const T*>(p.x);
-
-  Vec<T, V> vr[S], vx[S];
-  if (on) {
-    const long long b = col / p.Dw, d = col - b * p.Dw;
-    raw += t0 * p.raw_st + b * p.raw_sb + d;
-    x += t0 * p.x_st + b * p.x_sb + d;
-  }
+template <typename T, int V>
+__device__ __forceinline__ Cols<V> widen(const Vec<T, V>& v) {
+  Cols<V> o;
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if (on && t0 + s < p.T) {
-      vr[s] = load_vec<T, V>(raw + s * p.raw_st);
-      vx[s] = load_vec<T, V>(x + s * p.x_st);
+  for (int i = 0; i < V; ++i) o[i] = Elem<T>::to_f32(v.v[i]);
+  return o;
+}
+// A thread's inputs in shared memory: slot (stream, step) of B bytes = V elements.
+template <typename T, int V, int S>
+struct Stage {
+  static constexpr int B = sizeof(T) * V;
+  static constexpr int kSlot = B < 4 ? 4 : B;  // (a slot also takes an fp32 intermediate)
+  static constexpr int kStream = S * kThreads * kSlot;  // bytes of one stream's rows
+  char* base;
+  __device__ __forceinline__ char* slot(int stream, int s) const {
+    return base + ((stream * S + s) * kThreads + threadIdx.x) * kSlot;
+  }
+  // Rows of one stream, from its element in row t0. Copies of 4 bytes and more run asynchronously; single 16-bit
+  // elements go through registers. Rows beyond T read as zeros.
+  __device__ __forceinline__ void fill(int stream, const T* at, long long stride, int rows) const {
+    if constexpr (B >= 4) {
+      const uint32_t to = smem_u32(slot(stream, 0));
+      if (rows >= S) {
+#pragma unroll
+        for (int s = 0; s < S; ++s, at += stride)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to + s * kThreads * kSlot), "l"(at), "n"(B) : "memory");
+      } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to + s * kThreads * kSlot),
+                       "l"(s < rows ? at + s * stride : at), "n"(B), "r"(s < rows ? B : 0)
+                       : "memory");
+      }
     } else {
+      T v[S];
 #pragma unroll
-      for (int v = 0; v < V; ++v) vr[s].v[v] = vx[s].v[v] = Elem<T>::zero();
+      for (int s = 0; s < S; ++s) v[s] = s < rows ? at[s * stride] : Elem<T>::zero();
+#pragma unroll
+      for (int s = 0; s < S; ++s) *reinterpret_cast<T*>(slot(stream, s)) = v[s];
     }
   }
-  float bias[V];
+  __device__ __forceinline__ Cols<V> get(int stream, int s) const { return widen<T, V>(*reinterpret_cast<const Vec<T, V>*>(slot(stream, s))); }
+  // V fp32 values of a step in its slots of the streams 0 and 1, as many in each as fit
+  static constexpr int kFloats = kSlot / 4;
+  __device__ __forceinline__ void put_f32(int s, const Cols<V>& c) const {
 #pragma unroll
-  for (int v = 0; v < V; ++v) bias[v] = (p.bias && on) ? p.bias[(col + v) % p.D] : 0.0f;
-  const Rows rows = row_kinds<S, PACKED>(p, t0, lane);
-  auto h0_at = [&](int s, float (&h)[V]) {
-    const int q = PACKED ? __shfl_sync(0xffffffffu, rows.seq, s) : 0;
+    for (int v = 0; v < V; v += kFloats) {
+      Vec<float, kFloats> q;
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = (p.h0 && on) ? p.h0[(long long)q * p.cols + col + v] : 0.0f;
-  };
-
-  float f[S][V], u[S][V];
-  MapV<V> mine;
-#pragma unroll
-  for (int v = 0; v < V; ++v) mine.P[v] = 1.0f, mine.H[v] = 0.0f;
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if ((rows.first >> s) & 1u) {
-      h0_at(s, mine.H);
-#pragma unroll
-      for (int v = 0; v < V; ++v) mine.P[v] = kCut;
+      for (int i = 0; i < kFloats; ++i) q.v[i] = c[v + i];
+      *reinterpret_cast<Vec<float, kFloats>*>(slot(v / kFloats, s)) = q;
     }
+  }
+  __device__ __forceinline__ Cols<V> get_f32(int s) const {
+    Cols<V> c;
+#pragma unroll
+    for (int v = 0; v < V; v += kFloats) {
+      const Vec<float, kFloats> q = *reinterpret_cast<const Vec<float, kFloats>*>(slot(v / kFloats, s));
+#pragma unroll
+      for (int i = 0; i < kFloats; ++i) c[v + i] = q.v[i];
+    }
+    return c;
+  }
+};
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> narrow(const Cols<V>& c) {
+  Vec<T, V> o;
+#pragma unroll
+  for (int v = 0; v < V; ++v) o.v[v] = Elem<T>::from_f32(c[v]);
+  return o;
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait_but_last() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// What a CTA works on: a block of columns in a chunk, the pos-th in the order of work. pos < 0: nothing is left.
+struct Tile {
+  int pos, block;
+};
+// A CTA's tiles. CHAIN: tickets, drawn by one thread and passed on at the barrier that every tile has. Where chunks
+// pass maps, the next one is drawn when a tile is begun, not earlier: tiles are then begun nearly in the order of
+// their numbers, and none that others wait for lies behind another tile in its own CTA (two drawn at the start
+// put every second one there: 450 us instead of 130 for 32768 x 768 bf16). With g = 1 only the block's own previous
+// chunk matters, long done, so tickets are drawn, and inputs copied, one tile further ahead. Without CHAIN there is
+// one chunk, and every CTA has its share of its blocks.
+template <bool CHAIN>
+struct Tickets {
+  Tile* shared;  // [2]
+  uint32_t drawn;
+  __device__ __forceinline__ Tile tile(const GatedParams& p) const {
+    const int pos = drawn / (uint32_t)p.nb;
+    return pos < p.nchunks ? Tile{pos, (int)(drawn - (uint32_t)pos * p.nb)} : Tile{-1, 0};
+  }
+  __device__ __forceinline__ Tile first(const GatedParams& p) {
+    if constexpr (CHAIN) return another(p);
+    drawn = blockIdx.x;
+    return Tile{0, (int)drawn};
+  }
+  __device__ __forceinline__ Tile another(const GatedParams& p) {
+    if constexpr (!CHAIN) return receive(p, 0);
+    draw(p);
+    pass_on(p, 1);
+    __syncthreads();
+    const Tile t = shared[1];
+    __syncthreads();
+    return t;
+  }
+  __device__ __forceinline__ void draw(const GatedParams& p) {
+    if constexpr (CHAIN)
+      if (threadIdx.x == 0) drawn = atomicAdd(p.ticket, 1u) + 1u;  // (the counter starts at 0xffffffff)
+  }
+  __device__ __forceinline__ void pass_on(const GatedParams& p, int parity) {
+    if constexpr (CHAIN)
+      if (threadIdx.x == 0) shared[parity] = tile(p);
+  }
+  __device__ __forceinline__ Tile receive(const GatedParams& p, int parity) {
+    if constexpr (CHAIN) return shared[parity];
+    drawn += gridDim.x;
+    return drawn < (uint32_t)p.nb ? Tile{0, (int)drawn} : Tile{-1, 0};
+  }
+};
+
+__device__ __forceinline__ long long input_at(const GatedParams& p, int col, long long st, long long sb, int t0) {
+  if (p.Dw == p.cols) return t0 * st + col;
+  const int b = col / p.Dw;
+  return t0 * st + b * sb + (col - b * p.Dw);
+}
+template <int V>
+__device__ __forceinline__ Cols<V> load_bias(const GatedParams& p, int col, bool on) {
+  Cols<V> b = all<V>(0.0f);
+  if (p.bias && on) {
+    int d = p.D == p.cols ? col : col % p.D;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float m;
-      gate(Elem<T>::to_f32(vr[s].v[v]) + bias[v], f[s][v], m);
-      u[s][v] = m * Elem<T>::to_f32(vx[s].v[v]);
-      mine.P[v] *= f[s][v];
-      mine.H[v] = fmaf(f[s][v], mine.H[v], u[s][v]);
+      b[v] = __ldg(p.bias + d);
+      d = d + 1 == p.D ? 0 : d + 1;
     }
   }
-  maps[threadIdx.x] = mine;
-  __syncthreads();
-
-  // the warps of this column group: maps[(wc_idx * wt + i) * 32 + lane], i = 0 .. wt - 1 in time order
-  const int first_slot = wc_idx * wt * 32 + lane;
-  float h[V];
+  return b;
+}
+template <bool PACKED, int V>
+__device__ __forceinline__ Cols<V> state_at(const GatedParams& p, const float* from, const Rows& rows, int s, int col, bool on) {
+  const int q = PACKED ? __shfl_sync(0xffffffffu, rows.seq, s) : 0;
+  Cols<V> o;
 #pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = 0.0f;
-  if constexpr (CHAIN) {
-    const bool group_end = chunk % p.g == p.g - 1;
-    const bool more = chunk + 1 < p.nchunks;
-    MapV<V> all;
-    if (wt_idx == wt - 1 && more) {
-      all = maps[first_slot];
-      for (int i = 1; i < wt; ++i) {
-        const MapV<V> q = maps[first_slot + i * 32];
+  for (int v = 0; v < V; ++v) o[v] = (from && on) ? from[(long long)q * p.cols + col + v] : 0.0f;
+  return o;
+}
+template <bool PACKED, int V>
+__device__ __forceinline__ void put_state(const GatedParams& p, float* to, const Rows& rows, int s, int col, bool on,
+                                          const Cols<V>& o) {
+  const int q = PACKED ? __shfl_sync(0xffffffffu, rows.seq, s) : 0;
+  if (on && to)
 #pragma unroll
-        for (int v = 0; v < V; ++v) then_map(all.P[v], all.H[v], q.P[v], q.H[v]);
-      }
-      if (!group_end && on)
+    for (int v = 0; v < V; ++v) to[(long long)q * p.cols + col + v] = o[v];
+}
+// An empty sequence ends in the state that it starts from (and hands back what it is handed).
+template <int V>
+__device__ __forceinline__ void empty_sequences(const GatedParams& p, const float* from, float* to, int col, int wt_idx) {
+  if (to)
+    for (int q = wt_idx; q < p.S_seqs; q += p.wt)
+      if (__ldg(p.cu + q + 1) <= __ldg(p.cu + q))
 #pragma unroll
         for (int v = 0; v < V; ++v)
-          post64(p.maps + (long long)chunk * p.cols + col + v, publishable(all.P[v]), publishable(all.H[v]));
+          to[(long long)q * p.cols + col + v] = from ? from[(long long)q * p.cols + col + v] : 0.0f;
+}
+template <int V>
+__device__ __forceinline__ void post_map(const GatedParams& p, int pos, int col, const MapV<V>& m) {
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    post64(p.maps + (long long)pos * p.cols + col + v, publishable(m.P[v]), publishable(m.H[v]));
+}
+template <int V>
+__device__ __forceinline__ void post_state(const GatedParams& p, int pos, int col, const Cols<V>& h) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) post32(p.states + (long long)(pos / p.g) * p.cols + col + v, publishable(h[v]));
+}
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+template <typename T, int V, bool PACKED, bool CHAIN>
+__global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const GatedParams p) {
+  constexpr int S = kFwdSteps;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ MapV<V> maps[2][kThreads], part[CHAIN ? kThreads : 1];
+  __shared__ Tile s_tiles[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wt = p.wt, wt_idx = warp % wt, wc_idx = warp / wt;
+  const int first_slot = wc_idx * wt * 32 + lane;  // the warps of this column group: first_slot + 32 i in time order
+  const int my_col = wc_idx * (32 * V) + lane * V, width = 32 * V * (kWarps / wt);
+  auto stage = [&](int i) { return Stage<T, V, S>{smem + i * (2 * Stage<T, V, S>::kStream)}; };
+  auto fill = [&](const Tile t, const Stage<T, V, S> st, Cols<V>& bias) {
+    const int col = t.block * width + my_col, t0 = (t.pos * wt + wt_idx) * S;
+    const bool on = t.pos >= 0 && col < p.cols;
+    if (on) {
+      st.fill(0, static_cast<const T*>(p.raw) + input_at(p, col, p.raw_st, p.raw_sb, t0), p.raw_st, p.T - t0);
+      st.fill(1, static_cast<const T*>(p.x) + input_at(p, col, p.x_st, p.x_sb, t0), p.x_st, p.T - t0);
     }
-    chunk_start<V>(p, chunk, col, on, wt_idx, wt, part, threadIdx.x, h);
-    if (wt_idx == wt - 1 && more && group_end && on)
+    copies_commit();
+    bias = load_bias<V>(p, col, on);
+  };
+  Tickets<CHAIN> tickets{s_tiles};
+  Tile tile = tickets.first(p), next = {-1, 0};
+  Cols<V> bias, next_bias;
+  fill(tile, stage(0), bias);
+  const bool ahead = !CHAIN || p.g == 1;
+  if (ahead) next = tickets.another(p);
+
+  for (int parity = 0; tile.pos >= 0; parity ^= 1) {
+    if (ahead) fill(next, stage(parity ^ 1), next_bias);
+    tickets.draw(p);
+    const int col = tile.block * width + my_col, t0 = (tile.pos * wt + wt_idx) * S;
+    const bool on = col < p.cols;
+    Early<V> early;
+    if constexpr (CHAIN) early.look(p, tile.pos / p.g - 1, col, on && (p.g == 1 || wt_idx == 0));
+    const Rows rows = row_kinds<S, PACKED>(p, t0, lane);
+    const bool plain = rows.plain(S);
+    const Stage<T, V, S> in = stage(parity);
+    if (ahead) copies_wait_but_last(); else copies_wait();
+    bias = mul<V>(bias, all<V>(-kLog2e));
+
+    Cols<V> f[S], u[S];
+    MapV<V> mine = {all<V>(1.0f), all<V>(0.0f)};
+    auto local = [&](auto special) {
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        post32(p.states + (long long)(chunk / p.g) * p.cols + col + v, publishable(apply_map(all.P[v], all.H[v], h[v])));
-    if (p.ckpt && wt_idx == 0 && on)
-#pragma unroll
-      for (int v = 0; v < V; ++v) p.ckpt[(long long)chunk * p.cols + col + v] = h[v];
-  }
-  for (int i = 0; i < wt_idx; ++i) {
-    const MapV<V> q = maps[first_slot + i * 32];
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = apply_map(q.P[v], q.H[v], h[v]);
-  }
-  T* y = static_cast<T*>(p.y) + t0 * p.cols + col;
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if ((rows.first >> s) & 1u) h0_at(s, h);
-    Vec<T, V> o;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      h[v] = fmaf(f[s][v], h[v], u[s][v]);
-      o.v[v] = ((rows.in >> s) & 1u) ? Elem<T>::from_f32(h[v]) : Elem<T>::zero();
+      for (int s = 0; s < S; ++s) {
+        if constexpr (decltype(special)::value)
+          if ((rows.first >> s) & 1u) mine = {all<V>(kCut), state_at<PACKED, V>(p, p.h0, rows, s, col, on)};
+        Cols<V> m;
+        gate<V>(in.get(0, s), bias, f[s], m);
+        u[s] = mul<V>(m, in.get(1, s));
+        mine.P = mul<V>(mine.P, f[s]);
+        mine.H = fma<V>(f[s], mine.H, u[s]);
+      }
+    };
+    if (plain) local(No()); else local(Yes());
+    maps[parity][threadIdx.x] = mine;
+    tickets.pass_on(p, parity);
+    __syncthreads();
+    const Tile drawn = tickets.receive(p, parity);
+    if (!ahead) fill(next = drawn, stage(parity ^ 1), next_bias);
+
+    Cols<V> h = all<V>(0.0f);
+    const bool speaker = CHAIN && wt_idx == wt - 1 && on && tile.pos + 1 < p.nchunks;
+    const bool group_end = CHAIN && tile.pos % p.g == p.g - 1;
+    if constexpr (CHAIN) {
+      if (speaker && !group_end) {
+        MapV<V> whole = maps[parity][first_slot];
+        for (int i = 1; i < wt; ++i) then_map<PACKED, V>(whole, maps[parity][first_slot + i * 32].P, maps[parity][first_slot + i * 32].H);
+        post_map<V>(p, tile.pos, col, whole);
+      }
+      h = chunk_start<PACKED, V>(p, early, tile.pos, col, on, wt_idx, wt, part, first_slot);
     }
-    if (on && t0 + s < p.T) *reinterpret_cast<Vec<T, V>*>(y + s * p.cols) = o;
-    if ((rows.last >> s) & 1u) {
-      const int q = PACKED ? __shfl_sync(0xffffffffu, rows.seq, s) : 0;
-      if (on)
+    for (int i = 0; i < wt_idx; ++i) h = apply_map<PACKED, V>(maps[parity][first_slot + i * 32].P, maps[parity][first_slot + i * 32].H, h);
+    if (p.ckpt && t0 % kCkptRows == 0 && t0 < p.T && on)
 #pragma unroll
-        for (int v = 0; v < V; ++v) p.h_last[(long long)q * p.cols + col + v] = h[v];
-    }
-  }
-  if constexpr (PACKED) {  // an empty sequence ends in the state that it starts from
-    if (chunk == 0 && on)
-      for (int q = wt_idx; q < p.S_seqs; q += wt)
-        if (p.cu[q + 1] <= p.cu[q])
+      for (int v = 0; v < V; ++v) p.ckpt[(long long)(t0 / kCkptRows) * p.cols + col + v] = h[v];
+    if (speaker && group_end) post_state<V>(p, tile.pos, col, apply_map<PACKED, V>(mine.P, mine.H, h));
+    T* y = static_cast<T*>(p.y) + (long long)t0 * p.cols + col;
+    auto run = [&](auto special) {
 #pragma unroll
-          for (int v = 0; v < V; ++v)
-            p.h_last[(long long)q * p.cols + col + v] = p.h0 ? p.h0[(long long)q * p.cols + col + v] : 0.0f;
+      for (int s = 0; s < S; ++s, y += p.cols) {
+        if constexpr (decltype(special)::value)
+          if ((rows.first >> s) & 1u) h = state_at<PACKED, V>(p, p.h0, rows, s, col, on);
+        h = fma<V>(f[s], h, u[s]);
+        if constexpr (decltype(special)::value) {
+          if (on && t0 + s < p.T)
+            *reinterpret_cast<Vec<T, V>*>(y) = narrow<T, V>(((rows.in >> s) & 1u) ? h : all<V>(0.0f));
+          if ((rows.last >> s) & 1u) put_state<PACKED, V>(p, p.h_last, rows, s, col, on, h);
+        } else {
+          if (on) *reinterpret_cast<Vec<T, V>*>(y) = narrow<T, V>(h);
+        }
+      }
+    };
+    if (plain) run(No()); else run(Yes());
+    if constexpr (PACKED)
+      if (tile.pos == 0 && on) empty_sequences<V>(p, p.h0, p.h_last, col, wt_idx);
+    tile = next;
+    next = drawn;
+    bias = next_bias;
   }
 }
 
 // Reverse pass of a chunk. Both directions need only the products of f and a partial sum each, so one exchange
 // carries them: (P, H) takes a state forward through a warp's steps (the forward's states are computed again
-// from the chunk's saved starting state), (P, K) takes the hand-back through them in reverse.
+// from the chunk's saved starting state), (P, K) takes the hand-back through them in reverse. f and 1 - f stay in
+// registers, x and dy in shared memory, and h_{t-1} - x_t takes the place of raw and x there. The exchange has one
+// buffer and a barrier before it is written again.
 template <int V>
 struct TripleV {
-  float P[V], H[V], K[V];
+  Cols<V> P, H, K;
 };
 
-template <typename T, int V, int S, bool PACKED, bool CHAIN>
-__global__ void __launch_bounds__(kThreads) gated_bwd_kernel(const GatedParams p) {
+template <typename T, int V, bool PACKED, bool CHAIN>
+__global__ void __launch_bounds__(kThreads, 3) gated_bwd_kernel(const GatedParams p) {
+  constexpr int S = kBwdSteps;
+  extern __shared__ __align__(16) char smem[];
   __shared__ TripleV<V> trip[kThreads];
-  __shared__ MapV<V> part[CHAIN ? kThreads : 1];
-  __shared__ uint32_t s_ticket;
+  __shared__ Cols<V> s_db[kThreads];
+  __shared__ Tile s_tiles[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int wt = p.wt, wt_idx = warp % wt, wc_idx = warp / wt, wc = kWarps / wt;
-  long long work = blockIdx.x;
-  if constexpr (CHAIN) {
-    if (threadIdx.x == 0) s_ticket = atomicAdd(p.ticket, 1u) + 1u;
-    __syncthreads();
-    work = s_ticket;
-  }
-  const int pos = (int)(work / p.nb), chunk = p.nchunks - 1 - pos;
-  const long long col = ((work % p.nb) * wc + wc_idx) * (32 * V) + (long long)lane * V;
-  const bool on = col < p.cols;
-  const long long t0 = ((long long)chunk * wt + wt_idx) * S;
-  const T* raw = static_cast<const T*>(p.raw);
-  const T* x = static_cast<const T*>(p.x);
-  const T* dy = static_cast<const T*>(p.dy);
-
-  Vec<T, V> vr[S], vx[S], vg[S];
-  if (on) {
-    const long long b = col / p.Dw, d = col - b * p.Dw;
-    raw += t0 * p.raw_st + b * p.raw_sb + d;
-    x += t0 * p.x_st + b * p.x_sb + d;
-    dy += t0 * p.cols + col;
-  }
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if (on && t0 + s < p.T) {
-      vr[s] = load_vec<T, V>(raw + s * p.raw_st);
-      vx[s] = load_vec<T, V>(x + s * p.x_st);
-      vg[s] = load_vec<T, V>(dy + s * p.cols);
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) vr[s].v[v] = vx[s].v[v] = vg[s].v[v] = Elem<T>::zero();
-    }
-  }
-  float bias[V], h[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    bias[v] = (p.bias && on) ? p.bias[(col + v) % p.D] : 0.0f;
-    h[v] = (CHAIN && on) ? p.ckpt[(long long)chunk * p.cols + col + v] : 0.0f;
-  }
-  const Rows rows = row_kinds<S, PACKED>(p, t0, lane);
-  auto state_at = [&](const float* from, int s, float (&o)[V]) {
-    const int q = PACKED ? __shfl_sync(0xffffffffu, rows.seq, s) : 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = (from && on) ? from[(long long)q * p.cols + col + v] : 0.0f;
-  };
-
-  float gt[S][V];
-  TripleV<V> mine;
-#pragma unroll
-  for (int v = 0; v < V; ++v) mine.P[v] = 1.0f, mine.H[v] = 0.0f, mine.K[v] = 0.0f;
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if ((rows.first >> s) & 1u) state_at(p.h0, s, mine.H);
-    // a state does not pass a sequence's border in either direction: one product serves both
-    const bool cut = ((rows.first | rows.last | ~rows.in) >> s) & 1u;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float f, m;
-      gt[s][v] = gate_packed(Elem<T>::to_f32(vr[s].v[v]) + bias[v]);
-      gate_unpack(gt[s][v], f, m);
-      mine.H[v] = fmaf(f, mine.H[v], m * Elem<T>::to_f32(vx[s].v[v]));
-      mine.P[v] = cut ? kCut : mine.P[v] * f;
-    }
-  }
-#pragma unroll
-  for (int s = S - 1; s >= 0; --s) {
-    if ((rows.last >> s) & 1u) state_at(p.dh_last, s, mine.K);
-    const bool in = (rows.in >> s) & 1u;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float f, m;
-      gate_unpack(gt[s][v], f, m);
-      mine.K[v] = in ? f * (mine.K[v] + Elem<T>::to_f32(vg[s].v[v])) : 0.0f;
-    }
-  }
-  trip[threadIdx.x] = mine;
-  __syncthreads();
-
+  const int wt = p.wt, wt_idx = warp % wt, wc_idx = warp / wt;
   const int first_slot = wc_idx * wt * 32 + lane;
-  float K[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) K[v] = 0.0f;
-  if constexpr (CHAIN) {
-    const bool group_end = pos % p.g == p.g - 1;
-    const bool more = chunk > 0;
-    MapV<V> all;
-    if (wt_idx == 0 && more) {
-      const TripleV<V> l = trip[first_slot + (wt - 1) * 32];
-#pragma unroll
-      for (int v = 0; v < V; ++v) all.P[v] = l.P[v], all.H[v] = l.K[v];
-      for (int i = wt - 2; i >= 0; --i) {
-        const TripleV<V> q = trip[first_slot + i * 32];
-#pragma unroll
-        for (int v = 0; v < V; ++v) then_map(all.P[v], all.H[v], q.P[v], q.K[v]);
-      }
-      if (!group_end && on)
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          post64(p.maps + (long long)pos * p.cols + col + v, publishable(all.P[v]), publishable(all.H[v]));
+  const int my_col = wc_idx * (32 * V) + lane * V, width = 32 * V * (kWarps / wt);
+  auto stage = [&](int i) { return Stage<T, V, S>{smem + i * (3 * Stage<T, V, S>::kStream)}; };
+  auto fill = [&](const Tile t, const Stage<T, V, S> st, Cols<V>& bias, Cols<V>& ckpt) {
+    const int chunk = p.nchunks - 1 - t.pos, col = t.block * width + my_col, t0 = (chunk * wt + wt_idx) * S;
+    const bool on = t.pos >= 0 && col < p.cols;
+    if (on) {
+      st.fill(0, static_cast<const T*>(p.raw) + input_at(p, col, p.raw_st, p.raw_sb, t0), p.raw_st, p.T - t0);
+      st.fill(1, static_cast<const T*>(p.x) + input_at(p, col, p.x_st, p.x_sb, t0), p.x_st, p.T - t0);
+      st.fill(2, static_cast<const T*>(p.dy) + (long long)t0 * p.cols + col, p.cols, p.T - t0);
     }
-    chunk_start<V>(p, pos, col, on, wt_idx, wt, part, threadIdx.x, K);
-    if (wt_idx == 0 && more && group_end && on)
+    copies_commit();
+    bias = load_bias<V>(p, col, on);
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        post32(p.states + (long long)(pos / p.g) * p.cols + col + v, publishable(apply_map(all.P[v], all.H[v], K[v])));
-  }
-  for (int i = 0; i < wt_idx; ++i) {
-    const TripleV<V> q = trip[first_slot + i * 32];
+    for (int v = 0; v < V; ++v) ckpt[v] = (on && p.ckpt) ? __ldg(p.ckpt + (long long)chunk * p.cols + col + v) : 0.0f;
+  };
+  // the sum over a tile's steps of d_raw, added up in the order of the warps one barrier later
+  auto bias_sum = [&](const Tile t) {
+    const int col = t.block * width + my_col;
+    if (p.d_bias_part && wt_idx == 0 && col < p.cols) {
+      Cols<V> sum = s_db[first_slot];
+      for (int i = 1; i < wt; ++i) sum = add<V>(sum, s_db[first_slot + i * 32]);
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = apply_map(q.P[v], q.H[v], h[v]);
-  }
-  for (int i = wt - 1; i > wt_idx; --i) {
-    const TripleV<V> q = trip[first_slot + i * 32];
-#pragma unroll
-    for (int v = 0; v < V; ++v) K[v] = apply_map(q.P[v], q.K[v], K[v]);
-  }
+      for (int v = 0; v < V; ++v) p.d_bias_part[(long long)(p.nchunks - 1 - t.pos) * p.cols + col + v] = sum[v];
+    }
+  };
+  Tickets<CHAIN> tickets{s_tiles};
+  Tile tile = tickets.first(p), next = {-1, 0}, before = {-1, 0};
+  Cols<V> bias, next_bias, h, next_h;
+  fill(tile, stage(0), bias, h);
+  const bool ahead = !CHAIN || p.g == 1;
+  if (ahead) next = tickets.another(p);
 
-  float d[S][V];  // h_{t-1} - x_t
+  for (int parity = 0; tile.pos >= 0; parity ^= 1) {
+    if (ahead) fill(next, stage(parity ^ 1), next_bias, next_h);
+    tickets.draw(p);
+    const int chunk = p.nchunks - 1 - tile.pos, col = tile.block * width + my_col, t0 = (chunk * wt + wt_idx) * S;
+    const bool on = col < p.cols;
+    Early<V> early;
+    if constexpr (CHAIN) early.look(p, tile.pos / p.g - 1, col, on && (p.g == 1 || wt_idx == 0));
+    const Rows rows = row_kinds<S, PACKED>(p, t0, lane);
+    const bool plain = rows.plain(S);
+    const Stage<T, V, S> in = stage(parity);
+    if (ahead) copies_wait_but_last(); else copies_wait();
+    bias = mul<V>(bias, all<V>(-kLog2e));
+
+    Cols<V> f[S], m[S];
+    TripleV<V> mine = {all<V>(1.0f), all<V>(0.0f), all<V>(0.0f)};
+    auto local = [&](auto special) {
+      constexpr bool kSpecial = decltype(special)::value;
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if ((rows.first >> s) & 1u) state_at(p.h0, s, h);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float xv = Elem<T>::to_f32(vx[s].v[v]);
-      float f, m;
-      gate_unpack(gt[s][v], f, m);
-      d[s][v] = h[v] - xv;
-      h[v] = fmaf(f, h[v], m * xv);
-    }
-  }
-  float db[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) db[v] = 0.0f;
-  T* o_raw = static_cast<T*>(p.d_raw) + t0 * p.cols + col;
-  T* o_x = static_cast<T*>(p.d_x) + t0 * p.cols + col;
-#pragma unroll
-  for (int s = S - 1; s >= 0; --s) {
-    if ((rows.last >> s) & 1u) state_at(p.dh_last, s, K);
-    const bool in = (rows.in >> s) & 1u;
-    Vec<T, V> a, c;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float G = K[v] + Elem<T>::to_f32(vg[s].v[v]);
-      float f, m;
-      gate_unpack(gt[s][v], f, m);
-      K[v] = f * G;
-      const float g_x = in ? m * G : 0.0f, g_a = in ? K[v] * m * d[s][v] : 0.0f;
-      db[v] += g_a;
-      a.v[v] = Elem<T>::from_f32(g_a);
-      c.v[v] = Elem<T>::from_f32(g_x);
-    }
-    if (on && t0 + s < p.T) {
-      if (p.d_raw) *reinterpret_cast<Vec<T, V>*>(o_raw + s * p.cols) = a;
-      if (p.d_x) *reinterpret_cast<Vec<T, V>*>(o_x + s * p.cols) = c;
-    }
-    if (((rows.first >> s) & 1u) && p.d_h0) {
-      const int q = PACKED ? __shfl_sync(0xffffffffu, rows.seq, s) : 0;
-      if (on)
-#pragma unroll
-        for (int v = 0; v < V; ++v) p.d_h0[(long long)q * p.cols + col + v] = K[v];
-    }
-  }
-  if (p.d_bias_part) {  // this chunk's sum over time, in the order of the warps
-    __syncthreads();
-    float* acc = reinterpret_cast<float*>(trip);
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[threadIdx.x * V + v] = db[v];
-    __syncthreads();
-    if (wt_idx == 0 && on)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float sum = 0.0f;
-        for (int i = 0; i < wt; ++i) sum += acc[(first_slot + i * 32) * V + v];
-        p.d_bias_part[(long long)chunk * p.cols + col + v] = sum;
+      for (int s = 0; s < S; ++s) {
+        if constexpr (kSpecial)
+          if ((rows.first >> s) & 1u) mine.H = state_at<PACKED, V>(p, p.h0, rows, s, col, on);
+        gate<V>(in.get(0, s), bias, f[s], m[s]);
+        mine.H = fma<V>(f[s], mine.H, mul<V>(m[s], in.get(1, s)));
+        mine.P = mul<V>(mine.P, f[s]);
+        // a state does not pass a sequence's border in either direction: one product serves both
+        if constexpr (kSpecial)
+          if (((rows.first | rows.last | ~rows.in) >> s) & 1u) mine.P = all<V>(kCut);
       }
-  }
-  if constexpr (PACKED) {
-    if (chunk == 0 && on && p.d_h0)
-      for (int q = wt_idx; q < p.S_seqs; q += wt)
-        if (p.cu[q + 1] <= p.cu[q])
 #pragma unroll
-          for (int v = 0; v < V; ++v)
-            p.d_h0[(long long)q * p.cols + col + v] = p.dh_last ? p.dh_last[(long long)q * p.cols + col + v] : 0.0f;
+      for (int s = S - 1; s >= 0; --s) {
+        if constexpr (kSpecial)
+          if ((rows.last >> s) & 1u) mine.K = state_at<PACKED, V>(p, p.dh_last, rows, s, col, on);
+        mine.K = mul<V>(f[s], add<V>(mine.K, in.get(2, s)));
+        if constexpr (kSpecial)
+          if (!((rows.in >> s) & 1u)) mine.K = all<V>(0.0f);
+      }
+    };
+    if (plain) local(No()); else local(Yes());
+    tickets.pass_on(p, parity);
+    __syncthreads();  // the exchange of the tile before has been read
+    trip[threadIdx.x] = mine;
+    const Tile drawn = tickets.receive(p, parity);
+    if (!ahead) fill(next = drawn, stage(parity ^ 1), next_bias, next_h);
+    if (before.pos >= 0) bias_sum(before);
+    __syncthreads();
+
+    Cols<V> K = all<V>(0.0f);
+    const bool speaker = CHAIN && wt_idx == 0 && on && chunk > 0;
+    const bool group_end = CHAIN && tile.pos % p.g == p.g - 1;
+    if constexpr (CHAIN) {
+      if (speaker && !group_end) {
+        const TripleV<V>& l = trip[first_slot + (wt - 1) * 32];
+        MapV<V> whole = {l.P, l.K};
+        for (int i = wt - 2; i >= 0; --i) then_map<PACKED, V>(whole, trip[first_slot + i * 32].P, trip[first_slot + i * 32].K);
+        post_map<V>(p, tile.pos, col, whole);
+      }
+    }
+    for (int i = 0; i < wt_idx; ++i) h = apply_map<PACKED, V>(trip[first_slot + i * 32].P, trip[first_slot + i * 32].H, h);
+    MapV<V> behind = {all<V>(1.0f), all<V>(0.0f)};  // what lies between this warp's steps and the chunk's end
+    for (int i = wt - 1; i > wt_idx; --i) then_map<PACKED, V>(behind, trip[first_slot + i * 32].P, trip[first_slot + i * 32].K);
+    if constexpr (CHAIN) {
+      if (p.g > 1) __syncthreads();  // the parts of the starting state take the place of the exchange
+      K = chunk_start<PACKED, V>(p, early, tile.pos, col, on, wt_idx, wt, reinterpret_cast<MapV<V>*>(trip), first_slot);
+    }
+    K = apply_map<PACKED, V>(behind.P, behind.H, K);
+    if (speaker && group_end) post_state<V>(p, tile.pos, col, apply_map<PACKED, V>(mine.P, mine.K, K));
+
+    Cols<V> db = all<V>(0.0f);
+    auto run = [&](auto special) {
+      constexpr bool kSpecial = decltype(special)::value;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if constexpr (kSpecial)
+          if ((rows.first >> s) & 1u) h = state_at<PACKED, V>(p, p.h0, rows, s, col, on);
+        const Cols<V> x = in.get(1, s);
+        const Cols<V> d = fma<V>(x, all<V>(-1.0f), h);
+        in.put_f32(s, d);
+        h = fma<V>(f[s], h, mul<V>(m[s], x));
+      }
+      T* o_raw = static_cast<T*>(p.d_raw) + (long long)(t0 + S - 1) * p.cols + col;
+      T* o_x = static_cast<T*>(p.d_x) + (long long)(t0 + S - 1) * p.cols + col;
+#pragma unroll
+      for (int s = S - 1; s >= 0; --s, o_raw -= p.cols, o_x -= p.cols) {
+        if constexpr (kSpecial)
+          if ((rows.last >> s) & 1u) K = state_at<PACKED, V>(p, p.dh_last, rows, s, col, on);
+        const Cols<V> d = in.get_f32(s);
+        const Cols<V> G = add<V>(K, in.get(2, s));
+        K = mul<V>(f[s], G);
+        Cols<V> g_x = mul<V>(m[s], G), g_a = mul<V>(mul<V>(K, m[s]), d);
+        if constexpr (kSpecial)
+          if (!((rows.in >> s) & 1u)) g_x = g_a = all<V>(0.0f);
+        db = add<V>(db, g_a);
+        if (on && (!kSpecial || t0 + s < p.T)) {
+          if (p.d_raw) *reinterpret_cast<Vec<T, V>*>(o_raw) = narrow<T, V>(g_a);
+          if (p.d_x) *reinterpret_cast<Vec<T, V>*>(o_x) = narrow<T, V>(g_x);
+        }
+        if constexpr (kSpecial)
+          if ((rows.first >> s) & 1u) put_state<PACKED, V>(p, p.d_h0, rows, s, col, on, K);
+      }
+    };
+    if (plain) run(No()); else run(Yes());
+    s_db[threadIdx.x] = db;
+    if constexpr (PACKED)
+      if (chunk == 0 && on) empty_sequences<V>(p, p.dh_last, p.d_h0, col, wt_idx);
+    before = tile;
+    tile = next;
+    next = drawn;
+    bias = next_bias;
+    h = next_h;
   }
+  __syncthreads();
+  if (before.pos >= 0) bias_sum(before);
 }
 
 // d_bias[d] = sum over rows of part[row][d], in 64 bits, in a fixed order: thread (i, j) of a CTA takes rows
@@ -575,105 +804,123 @@ __global__ void __launch_bounds__(256) gated_step_kernel(const T* __restrict__ r
   const long long dv = D / V, n = B * dv;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
     const long long b = i / dv, d = (i - b * dv) * V;
-    const Vec<T, V> vr = load_vec<T, V>(raw + b * raw_sb + d), vx = load_vec<T, V>(x + b * x_sb + d);
-    Vec<float, V> vh = load_vec<float, V>(h + b * D + d);
-    Vec<T, V> o;
+    const Vec<T, V> vr = *reinterpret_cast<const Vec<T, V>*>(raw + b * raw_sb + d);
+    const Vec<T, V> vx = *reinterpret_cast<const Vec<T, V>*>(x + b * x_sb + d);
+    Vec<float, V> vh = *reinterpret_cast<const Vec<float, V>*>(h + b * D + d);
+    Cols<V> c, f, m, hv;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float f, m;
-      gate(Elem<T>::to_f32(vr.v[v]) + (bias ? bias[d + v] : 0.0f), f, m);
-      vh.v[v] = fmaf(f, vh.v[v], m * Elem<T>::to_f32(vx.v[v]));
-      o.v[v] = Elem<T>::from_f32(vh.v[v]);
+      c[v] = bias ? gate_bias(bias[d + v]) : 0.0f;
+      hv[v] = vh.v[v];
     }
+    gate<V>(widen<T, V>(vr), c, f, m);
+    hv = fma<V>(f, hv, mul<V>(m, widen<T, V>(vx)));
+#pragma unroll
+    for (int v = 0; v < V; ++v) vh.v[v] = hv[v];
     *reinterpret_cast<Vec<float, V>*>(h + b * D + d) = vh;
-    *reinterpret_cast<Vec<T, V>*>(y + b * D + d) = o;
+    *reinterpret_cast<Vec<T, V>*>(y + b * D + d) = narrow<T, V>(hv);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host
 
-constexpr int kSteps = 8;  // steps of a warp's tile
-
 struct GatedPlan {
-  int wt, nchunks, g;
-  long long nb;
+  int wt, nchunks, g, nb;
 };
 
 // Warps of a CTA along time: as many as the steps need, up to all of them; the rest lie side by side over
-// the columns. Chunks hand on states one by one (g = 1) where a row of column blocks fills the GPU, so that
+// the columns. Chunks hand on states one by one (g = 1) where a row of column blocks occupies all CTAs, so that
 // a chunk's predecessor has finished long before; with fewer blocks, 32 chunks run side by side and pass maps.
-GatedPlan plan_gated(long long T, long long cols, int V, int sms) {
+GatedPlan plan_gated(long long T, long long cols, int V, int steps, long long ctas) {
   GatedPlan q;
   q.wt = 1;
-  while (q.wt < kWarps && (long long)q.wt * kSteps < T) q.wt *= 2;
-  const long long rows = (long long)q.wt * kSteps, width = 32LL * V * (kWarps / q.wt);
+  while (q.wt < kWarps && (long long)q.wt * steps < T) q.wt *= 2;
+  const long long rows = (long long)q.wt * steps, width = 32LL * V * (kWarps / q.wt);
   q.nchunks = (int)((T + rows - 1) / rows);
-  q.nb = (cols + width - 1) / width;
-  q.g = q.nb >= 3LL * sms ? 1 : 32;
+  q.nb = (int)((cols + width - 1) / width);
+  q.g = q.nb >= ctas ? 1 : 32;
   return q;
 }
-int chunk_rows(long long T) {
-  const GatedPlan q = plan_gated(T, 1, 1, 148);
-  return q.wt * kSteps;
-}
+// chunks of the backward, which are the smaller ones
+long long bwd_chunks(long long T) { return (T + kCkptRows - 1) / kCkptRows; }
+static_assert(kBwdSteps * kWarps == kCkptRows && kFwdSteps * kWarps >= kCkptRows && kCkptRows % kFwdSteps == 0, "");
 
 bool ok_dtype(int d) { return d == NSB_F32 || d == NSB_BF16 || d == NSB_F16; }
 bool fits(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 // scratch: [ticket, 3 words of padding][states][maps], filled with 0xff by one memset
 long long scratch_words(long long T, long long cols) {
-  const long long chunks = (T + chunk_rows(T) - 1) / chunk_rows(T);
+  const long long chunks = bwd_chunks(T);
   if (chunks <= 1) return 0;
   // whatever g the plan takes: all chunks' maps, or all chunks' states
   return 4 + ((chunks / 32 + 1) * cols + 3) / 4 * 4 + 2 * chunks * cols;
 }
 
-template <typename T>
-int launch_gated(GatedParams p, bool backward, uint32_t* scratch, cudaStream_t st) {
+template <typename T, int V, bool BACKWARD, bool PACKED, bool CHAIN>
+int start_kernel(const GatedParams& p, int ctas, int device, cudaStream_t st) {
+  const int smem = 2 * (BACKWARD ? 3 * Stage<T, V, kBwdSteps>::kStream : 2 * Stage<T, V, kFwdSteps>::kStream);
+  void (*kern)(const GatedParams);
+  if constexpr (BACKWARD) kern = gated_bwd_kernel<T, V, PACKED, CHAIN>;
+  else kern = gated_fwd_kernel<T, V, PACKED, CHAIN>;
+  static std::atomic<uint64_t> set_on{0};  // devices that know of the kernel's shared memory
+  const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+  if (!(set_on.load(std::memory_order_relaxed) & bit)) {
+    NSB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "shared memory of the gated recurrence");
+    set_on.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const unsigned grid = (unsigned)std::min<long long>((long long)p.nb * p.nchunks, ctas);
+  kern<<<grid, kThreads, smem, st>>>(p);
+  NSB_CUDA_TRY(cudaGetLastError(), BACKWARD ? "launch gated_bwd_kernel" : "launch gated_fwd_kernel");
+  return NSB_OK;
+}
+
+template <typename T, bool BACKWARD>
+int launch_gated(GatedParams p, uint32_t* scratch, cudaStream_t st) {
   DeviceInfo dev;
   int r = get_device_info(&dev);
   if (r != NSB_OK) return r;
-  int V = 2;
+  // 4 bytes of a row per lane: with 8 a warp's steps do not fit the registers as well (forward 16 steps x 4 bytes on
+  // two CTAs per SM against 8 x 8: 97 and 143 us for 8192 x 6144 columns bf16; backward 8 x 4 on three against 8 x 8
+  // on two: 194 and 226 us). One element where rows are not aligned to that or a warp would span all columns twice.
   auto all_fit = [&](int v) {
     const size_t a = sizeof(T) * v;
-    bool ok = p.Dw % v == 0 && p.raw_st % v == 0 && p.raw_sb % v == 0 && p.x_st % v == 0 && p.x_sb % v == 0 &&
-              p.cols % v == 0;
+    bool ok = p.cols % v == 0 && p.raw_st % v == 0 && p.x_st % v == 0;
+    if (p.Dw != p.cols) ok = ok && p.Dw % v == 0 && p.raw_sb % v == 0 && p.x_sb % v == 0;
     for (const void* q : {p.raw, p.x, p.dy, (const void*)p.y, (const void*)p.d_raw, (const void*)p.d_x})
       ok = ok && fits(q, a);
     return ok;
   };
-  while (V > 1 && !all_fit(V)) V /= 2;
-  const GatedPlan q = plan_gated(p.T, p.cols, V, dev.sm_count);
+  int V = 4 / (int)sizeof(T);
+  while (V > 1 && (!all_fit(V) || p.cols <= 16 * V)) V /= 2;
+  const int ctas = dev.sm_count * (BACKWARD ? 3 : 2);
+  const GatedPlan q = plan_gated(p.T, p.cols, V, BACKWARD ? kBwdSteps : kFwdSteps, ctas);
   p.nb = q.nb, p.nchunks = q.nchunks, p.g = q.g, p.wt = q.wt;
+  if ((long long)q.nb * q.nchunks > 0x7fffffffLL - 2 * ctas) return NSB_ERR_TOO_LARGE;
   const bool chain = q.nchunks > 1, packed = p.cu != nullptr;
   if (chain) {
     if (!scratch || !fits(scratch, 16)) return NSB_ERR_INVALID_ARG;
-    const long long nstates = (q.nchunks / q.g + 1) * p.cols;
+    const long long nstates = (q.nchunks / q.g + 1LL) * p.cols;
     const long long nmaps = q.g > 1 ? 2LL * q.nchunks * p.cols : 0;
     p.ticket = scratch;
     p.states = scratch + 4;
     p.maps = reinterpret_cast<uint2*>(scratch + 4 + (nstates + 3) / 4 * 4);
     NSB_CUDA_TRY(cudaMemsetAsync(scratch, 0xff, 4 * (4 + (nstates + 3) / 4 * 4 + nmaps), st), "memset gated scratch");
   }
-  const long long grid = q.nb * q.nchunks;
-  if (grid > 0x7fffffffLL) return NSB_ERR_TOO_LARGE;
-#define NSB_GO(V_, P_, C_)                                                                          \
-  (backward ? gated_bwd_kernel<T, V_, kSteps, P_, C_><<<(unsigned)grid, kThreads, 0, st>>>(p)       \
-            : gated_fwd_kernel<T, V_, kSteps, P_, C_><<<(unsigned)grid, kThreads, 0, st>>>(p))
-#define NSB_GO_V(V_) \
-  (packed ? (chain ? NSB_GO(V_, true, true) : NSB_GO(V_, true, false)) \
-          : (chain ? NSB_GO(V_, false, true) : NSB_GO(V_, false, false)))
-  if (V == 2) NSB_GO_V(2); else NSB_GO_V(1);
+#define NSB_GO_V(V_)                                                                           \
+  (packed ? (chain ? start_kernel<T, V_, BACKWARD, true, true>(p, ctas, dev.device, st)        \
+                   : start_kernel<T, V_, BACKWARD, true, false>(p, ctas, dev.device, st))      \
+          : (chain ? start_kernel<T, V_, BACKWARD, false, true>(p, ctas, dev.device, st)       \
+                   : start_kernel<T, V_, BACKWARD, false, false>(p, ctas, dev.device, st)))
+  if constexpr (sizeof(T) == 2)
+    if (V == 2) return NSB_GO_V(2);
+  return NSB_GO_V(1);
 #undef NSB_GO_V
-#undef NSB_GO
-  NSB_CUDA_TRY(cudaGetLastError(), backward ? "launch gated_bwd_kernel" : "launch gated_fwd_kernel");
-  return NSB_OK;
 }
 
 int check_sizes(int64_t T, int64_t B, int64_t D, int64_t seqs, const int32_t* cu, int dtype) {
   if (T < 0 || B < 0 || D < 0 || seqs < 0 || !ok_dtype(dtype)) return NSB_ERR_INVALID_ARG;
   if (cu ? (B != 1 || !fits(cu, 4)) : seqs != 0) return NSB_ERR_INVALID_ARG;
-  if (T > 0x7fffffffLL || seqs > 0x7ffffffeLL) return NSB_ERR_TOO_LARGE;
+  if (T > 0x7fffff00LL || seqs > 0x7ffffff0LL || (D > 0 && B > 0x7fffff00LL / D)) return NSB_ERR_TOO_LARGE;
   return NSB_OK;
 }
 
@@ -685,7 +932,7 @@ using namespace nsb;
 extern "C" int64_t nsb_gated_scratch_words(int64_t T, int64_t cols) {
   return T <= 0 || cols <= 0 ? 0 : scratch_words(T, cols);
 }
-extern "C" int64_t nsb_gated_chunks(int64_t T) { return T <= 0 ? 0 : (T + chunk_rows(T) - 1) / chunk_rows(T); }
+extern "C" int64_t nsb_gated_chunks(int64_t T) { return T <= 0 ? 0 : bwd_chunks(T); }
 
 extern "C" int nsb_gated_recurrence_fwd(const void* raw, int64_t raw_stride_t, int64_t raw_stride_b, const void* x,
                                         int64_t x_stride_t, int64_t x_stride_b, const float* bias, const float* h0,
@@ -710,14 +957,14 @@ extern "C" int nsb_gated_recurrence_fwd(const void* raw, int64_t raw_stride_t, i
   p.raw = raw, p.x = x, p.bias = bias, p.h0 = h0, p.cu = cu_seqlens, p.S_seqs = (int)seqs;
   p.y = y, p.h_last = h_last, p.ckpt = ckpt;
   p.raw_st = raw_stride_t, p.raw_sb = raw_stride_b, p.x_st = x_stride_t, p.x_sb = x_stride_b;
-  p.T = T, p.cols = cols, p.D = D;
-  p.Dw = (raw_stride_b == D && x_stride_b == D) || B == 1 ? cols : D;
+  p.T = (int)T, p.cols = (int)cols, p.D = (int)D;
+  p.Dw = (raw_stride_b == D && x_stride_b == D) || B == 1 ? p.cols : p.D;
   if (!(p.err = device_error_word_ptr())) return NSB_ERR_CUDA;
   p.limit_ns = get_wait_limit_ns();
   switch (dtype) {
-    case NSB_F32: return launch_gated<float>(p, false, scratch, st);
-    case NSB_BF16: return launch_gated<__nv_bfloat16>(p, false, scratch, st);
-    default: return launch_gated<__half>(p, false, scratch, st);
+    case NSB_F32: return launch_gated<float, false>(p, scratch, st);
+    case NSB_BF16: return launch_gated<__nv_bfloat16, false>(p, scratch, st);
+    default: return launch_gated<__half, false>(p, scratch, st);
   }
 }
 
@@ -754,14 +1001,14 @@ extern "C" int nsb_gated_recurrence_bwd(const void* raw, int64_t raw_stride_t, i
   p.S_seqs = (int)seqs, p.d_raw = d_raw, p.d_x = d_x, p.d_h0 = d_h0;
   p.ckpt = const_cast<float*>(ckpt), p.d_bias_part = d_bias ? bias_part : nullptr;
   p.raw_st = raw_stride_t, p.raw_sb = raw_stride_b, p.x_st = x_stride_t, p.x_sb = x_stride_b;
-  p.T = T, p.cols = cols, p.D = D;
-  p.Dw = (raw_stride_b == D && x_stride_b == D) || B == 1 ? cols : D;
+  p.T = (int)T, p.cols = (int)cols, p.D = (int)D;
+  p.Dw = (raw_stride_b == D && x_stride_b == D) || B == 1 ? p.cols : p.D;
   if (!(p.err = device_error_word_ptr())) return NSB_ERR_CUDA;
   p.limit_ns = get_wait_limit_ns();
   switch (dtype) {
-    case NSB_F32: r = launch_gated<float>(p, true, scratch, st); break;
-    case NSB_BF16: r = launch_gated<__nv_bfloat16>(p, true, scratch, st); break;
-    default: r = launch_gated<__half>(p, true, scratch, st);
+    case NSB_F32: r = launch_gated<float, true>(p, scratch, st); break;
+    case NSB_BF16: r = launch_gated<__nv_bfloat16, true>(p, scratch, st); break;
+    default: r = launch_gated<__half, true>(p, scratch, st);
   }
   if (r != NSB_OK || !d_bias) return r;
   NSB_CUDA_TRY(launch_dependent(gated_bias_kernel, dim3((unsigned)((D + 31) / 32)), dim3(1024), 0, st,

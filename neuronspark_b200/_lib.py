@@ -169,6 +169,25 @@ def stream_ptr(device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def address(t):
+    """Device address of a tensor as a plain integer (None stays None): what a c_void_p argument takes."""
+    return None if t is None else t.data_ptr()
+
+
+def launch(dev: torch.device, name: str, *args) -> None:
+    """Calls an entry point on the current stream of ``dev``, which is its last argument, with ``dev`` current.
+    A call that follows others on the same device costs neither a device switch nor a stream object (5 us a call)."""
+    fn = getattr(lib(), name)
+    index = dev.index
+    if index is None or torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(dev):
+            status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != NSB_OK:
+        check(status, name)
+
+
 def require_cuda(*tensors) -> torch.device:
     dev = None
     for t in tensors:

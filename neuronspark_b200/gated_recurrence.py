@@ -29,27 +29,27 @@ def _strided(t: torch.Tensor, dt: torch.dtype):
     already - half of a merged projection, say - is taken as it is."""
     if t.dtype != dt:
         return _lib.convert(t, dt)
-    t = t.detach()
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _view(t: torch.Tensor):
-    """(T, B, D, stride of t, stride of b) of a [T, B, D] or [T, D] tensor; further leading dimensions of a
-    state, as in ``linear_recurrence``, are folded into B (``t`` is contiguous then)."""
-    D = t.shape[-1]
-    if t.dim() == 2:
-        return t.shape[0], 1, D, t.stride(0), D
-    return t.shape[0], t.shape[1], D, t.stride(0), t.stride(1)
+def _sizes(t: torch.Tensor):
+    """(T, B, D) of a [T, B, D] or [T, D] tensor."""
+    return t.shape if t.dim() == 3 else (t.shape[0], 1, t.shape[1])
+
+
+def _strides(t: torch.Tensor):
+    """Strides of T and B in elements."""
+    s = t.stride()
+    return s[:2] if len(s) == 3 else (s[0], t.shape[1])
 
 
 def _f32(t, shape, what):
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise NSBError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype == torch.float32:
-        return t.detach().contiguous()
-    return t.detach().to(torch.float32).contiguous()
+    t = t.detach()
+    return t.contiguous() if t.dtype == torch.float32 else t.to(torch.float32).contiguous()
 
 
 class GatedLinearRecurrence(torch.autograd.Function):
@@ -57,60 +57,52 @@ class GatedLinearRecurrence(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, raw_gate, x, h0, bias, cu):
-        dt = _common_stream_dtype(raw_gate, x)
+        dt = x.dtype if raw_gate.dtype == x.dtype else _common_stream_dtype(raw_gate, x)
+        code = _lib.dtype_code(dt)
         a, v = _strided(raw_gate, dt), _strided(x, dt)
-        T, B, D, a_t, a_b = _view(a)
-        _, _, _, v_t, v_b = _view(v)
-        state = (cu.numel() - 1, D) if cu is not None else tuple(x.shape[1:])
-        h0_32, bias_32 = _f32(h0, state, "h0"), _f32(bias, (D,), "bias")
+        T, B, D = _sizes(x)
+        seqs = cu.shape[0] - 1 if cu is not None else 0
+        state = torch.Size((seqs, D)) if cu is not None else x.shape[1:]
+        h0_32, bias_32 = _f32(h0, state, "h0"), _f32(bias, x.shape[-1:], "bias")
         dev = _lib.require_cuda(a, v, h0_32, bias_32, cu)
-        L = _lib.lib()
+        L, at = _lib.lib(), _lib.address
         y = torch.empty(x.shape, dtype=dt, device=dev)
         h_last = torch.empty(state, dtype=torch.float32, device=dev)
         needs_grad = any(ctx.needs_input_grad)
-        chunks, words = int(L.nsb_gated_chunks(T)), int(L.nsb_gated_scratch_words(T, B * D))
+        chunks, words = L.nsb_gated_chunks(T), L.nsb_gated_scratch_words(T, B * D)
         ckpt = torch.empty(chunks * B * D, dtype=torch.float32, device=dev) if needs_grad and chunks > 1 else None
         scratch = torch.empty(words, dtype=torch.int32, device=dev) if words else None
-        seqs = cu.numel() - 1 if cu is not None else 0
-        p = _lib.ptr
-        with torch.cuda.device(dev):
-            _lib.check(L.nsb_gated_recurrence_fwd(
-                p(a), a_t, a_b, p(v), v_t, v_b, p(bias_32), p(h0_32), p(cu), seqs, p(y), p(h_last), p(ckpt), p(scratch),
-                T, B, D, _lib.dtype_code(dt), _lib.stream_ptr(dev)), "nsb_gated_recurrence_fwd")
+        _lib.launch(dev, "nsb_gated_recurrence_fwd", at(a), *_strides(a), at(v), *_strides(v), at(bias_32), at(h0_32),
+                    at(cu), seqs, at(y), at(h_last), at(ckpt), at(scratch), T, B, D, code)
         if needs_grad:
             ctx.save_for_backward(a, v, h0_32, bias_32, cu, ckpt)
-            ctx.in_dtypes = tuple(t.dtype if t is not None else None for t in (raw_gate, x, h0, bias))
+            ctx.in_dtypes = (raw_gate.dtype, x.dtype, h0.dtype if h0 is not None else None,
+                             bias.dtype if bias is not None else None)
             ctx.state = state
             ctx.set_materialize_grads(False)
-        return _cast(y, x.dtype), h_last
+        return (y if dt == x.dtype else _cast(y, x.dtype)), h_last
 
     @staticmethod
     def backward(ctx, dy, dh_last):
         a, v, h0, bias, cu, ckpt = ctx.saved_tensors
-        T, B, D, a_t, a_b = _view(a)
-        _, _, _, v_t, v_b = _view(v)
-        dev, dt, L = a.device, a.dtype, _lib.lib()
+        T, B, D = _sizes(v)
+        dev, dt, L, at = a.device, a.dtype, _lib.lib(), _lib.address
         dy = torch.zeros(v.shape, dtype=dt, device=dev) if dy is None else _lib.convert(dy, dt)
-        dh = None if dh_last is None else _lib.convert(dh_last, torch.float32)
-        want_a, want_x, want_h, want_b = ctx.needs_input_grad[:4]
+        dh = None if dh_last is None else dh_last.contiguous()
+        want_a, want_x, want_h, want_b, _ = ctx.needs_input_grad
         d_raw = torch.empty(a.shape, dtype=dt, device=dev) if want_a else None
         d_x = torch.empty(v.shape, dtype=dt, device=dev) if want_x else None
         d_h0 = torch.empty(ctx.state, dtype=torch.float32, device=dev) if want_h and h0 is not None else None
         d_bias = torch.empty(D, dtype=torch.float32, device=dev) if want_b and bias is not None else None
-        chunks, words = int(L.nsb_gated_chunks(T)), int(L.nsb_gated_scratch_words(T, B * D))
-        part = torch.empty(chunks * B * D, dtype=torch.float32, device=dev) if d_bias is not None else None
-        scratch = torch.empty(words, dtype=torch.int32, device=dev) if words else None
-        seqs = cu.numel() - 1 if cu is not None else 0
-        p = _lib.ptr
-        with torch.cuda.device(dev):
-            _lib.check(L.nsb_gated_recurrence_bwd(
-                p(a), a_t, a_b, p(v), v_t, v_b, p(bias), p(h0), p(cu), seqs, p(ckpt), p(dy), p(dh), p(d_raw), p(d_x),
-                p(d_bias), p(d_h0), p(part), p(scratch), T, B, D, _lib.dtype_code(dt), _lib.stream_ptr(dev)),
-                "nsb_gated_recurrence_bwd")
-        out = []
-        for g, t in zip((d_raw, d_x, d_h0, d_bias), ctx.in_dtypes):
-            out.append(g if g is None else _cast(g, t))
-        return (*out, None)
+        words = L.nsb_gated_scratch_words(T, B * D)  # (a multiple of 16 bytes)
+        sums = L.nsb_gated_chunks(T) * B * D if d_bias is not None else 0
+        scratch = torch.empty(words + sums, dtype=torch.float32, device=dev) if words + sums else None
+        part = scratch.data_ptr() + 4 * words if sums else None
+        _lib.launch(dev, "nsb_gated_recurrence_bwd", at(a), *_strides(a), at(v), *_strides(v), at(bias), at(h0), at(cu),
+                    cu.shape[0] - 1 if cu is not None else 0, at(ckpt), at(dy), at(dh), at(d_raw), at(d_x), at(d_bias),
+                    at(d_h0), part, at(scratch), T, B, D, _lib.dtype_code(dt))
+        return (*(g if g is None or g.dtype == t else _cast(g, t) for g, t in zip((d_raw, d_x, d_h0, d_bias), ctx.in_dtypes)),
+                None)
 
 
 def gated_linear_recurrence(raw_gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | None = None,
@@ -147,15 +139,15 @@ def gated_linear_recurrence_step(raw_gate: torch.Tensor, x: torch.Tensor, h: tor
         raise NSBError("gated_linear_recurrence_step expects raw_gate, x and h of one shape [B, D]")
     if h.dtype != torch.float32 or not h.is_contiguous():
         raise NSBError("gated_linear_recurrence_step: h must be a contiguous float32 tensor (it is updated in place)")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (raw_gate, x, h, bias)):
+    if torch.is_grad_enabled() and (raw_gate.requires_grad or x.requires_grad or h.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
         raise NSBError("gated_linear_recurrence_step has no gradients; use gated_linear_recurrence, or torch.no_grad()")
-    dt = _common_stream_dtype(raw_gate, x)
-    a, v, b = _strided(raw_gate, dt), _strided(x, dt), _f32(bias, (x.shape[1],), "bias")
+    dt = x.dtype if raw_gate.dtype == x.dtype else _common_stream_dtype(raw_gate, x)
+    code = _lib.dtype_code(dt)
+    a, v, b = _strided(raw_gate, dt), _strided(x, dt), _f32(bias, x.shape[1:], "bias")
     dev = _lib.require_cuda(a, v, h, b)
     y = torch.empty(x.shape, dtype=dt, device=dev)
-    p = _lib.ptr
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().nsb_gated_recurrence_step(
-            p(a), a.stride(0), p(v), v.stride(0), p(b), p(h), p(y), x.shape[0], x.shape[1], _lib.dtype_code(dt),
-            _lib.stream_ptr(dev)), "nsb_gated_recurrence_step")
-    return _cast(y, x.dtype)
+    at = _lib.address
+    _lib.launch(dev, "nsb_gated_recurrence_step", at(a), a.stride(0), at(v), v.stride(0), at(b), at(h), at(y), x.shape[0],
+                x.shape[1], code)
+    return y if dt == x.dtype else _cast(y, x.dtype)

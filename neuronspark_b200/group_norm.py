@@ -21,49 +21,53 @@ _ACTIVATIONS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU}
 
 
 def _param(t):
-    return None if t is None else t.detach().to(torch.float32).contiguous()
+    if t is None:
+        return None
+    t = t.detach()
+    return t.contiguous() if t.dtype == torch.float32 else t.to(torch.float32).contiguous()
 
 
 class GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, num_groups, eps, act):
-        x_c, w, b = x.detach().contiguous(), _param(weight), _param(bias)
+        x_c, w, b = x.contiguous(), _param(weight), _param(bias)
         dev = _lib.require_cuda(x_c, w, b)
-        N, C = x.shape[0], x.shape[-1]
-        L = x.numel() // (N * C) if N * C else 0
-        lib, code, p = _lib.lib(), _lib.dtype_code(x.dtype), _lib.ptr
-        y = torch.empty_like(x_c)
+        shape = x.shape
+        N, C = shape[0], shape[-1]
+        L = x_c.numel() // (N * C) if N * C else 0
+        lib, at = _lib.lib(), _lib.address
+        y = torch.empty(shape, dtype=x.dtype, device=dev)
         needs_grad = any(ctx.needs_input_grad)
-        stats = torch.empty((2, N, num_groups), dtype=torch.float32, device=dev) if needs_grad else (None, None)
-        words = int(lib.nsb_group_norm_scratch_floats(N, L, C, num_groups, 0))
+        stats = torch.empty(2 * N * num_groups, dtype=torch.float32, device=dev) if needs_grad else None
+        words = lib.nsb_group_norm_scratch_floats(N, L, C, num_groups, 0)
         scratch = torch.empty(words, dtype=torch.float32, device=dev) if words else None
-        with torch.cuda.device(dev):
-            _lib.check(lib.nsb_group_norm_fwd(p(x_c), p(w), p(b), p(y), p(stats[0]), p(stats[1]), p(scratch), N, L, C,
-                                              num_groups, eps, act, code, _lib.stream_ptr(dev)), "nsb_group_norm_fwd")
+        mean = at(stats)
+        rstd = mean + 4 * N * num_groups if mean else None
+        _lib.launch(dev, "nsb_group_norm_fwd", at(x_c), at(w), at(b), at(y), mean, rstd, at(scratch), N, L, C, num_groups,
+                    eps, act, _lib.dtype_code(x.dtype))
         if needs_grad:
             ctx.save_for_backward(x_c, w, b, stats)
             ctx.sizes = (N, L, C, num_groups, act)
-            ctx.in_dtypes = tuple(t.dtype if t is not None else None for t in (weight, bias))
+            ctx.in_dtypes = (weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
         return y
 
     @staticmethod
     def backward(ctx, grad_out):
         x, w, b, stats = ctx.saved_tensors
         N, L, C, G, act = ctx.sizes
-        dev, lib, p = x.device, _lib.lib(), _lib.ptr
+        dev, lib, at = x.device, _lib.lib(), _lib.address
         dy = _lib.convert(grad_out, x.dtype)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty_like(x) if need_x else None
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         dw = torch.empty(C, dtype=torch.float32, device=dev) if need_w and w is not None else None
         db = torch.empty(C, dtype=torch.float32, device=dev) if need_b and b is not None else None
-        words = int(lib.nsb_group_norm_scratch_floats(N, L, C, G, 1))
+        words = lib.nsb_group_norm_scratch_floats(N, L, C, G, 1)
         scratch = torch.empty(words, dtype=torch.float32, device=dev) if words else None
-        with torch.cuda.device(dev):
-            _lib.check(lib.nsb_group_norm_bwd(p(dy), p(x), p(w), p(b), p(stats[0]), p(stats[1]), p(dx), p(dw), p(db),
-                                              p(scratch), N, L, C, G, act, _lib.dtype_code(x.dtype), _lib.stream_ptr(dev)),
-                       "nsb_group_norm_bwd")
-        dw, db = (None if g is None else g.to(t) for g, t in zip((dw, db), ctx.in_dtypes))
-        return dx, dw, db, None, None, None
+        mean = at(stats)
+        rstd = mean + 4 * N * G if mean else None
+        _lib.launch(dev, "nsb_group_norm_bwd", at(dy), at(x), at(w), at(b), mean, rstd, at(dx), at(dw), at(db), at(scratch),
+                    N, L, C, G, act, _lib.dtype_code(x.dtype))
+        return (dx, *(g if g is None or g.dtype == t else g.to(t) for g, t in zip((dw, db), ctx.in_dtypes)), None, None, None)
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,

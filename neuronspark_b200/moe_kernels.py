@@ -151,14 +151,11 @@ def moe_few_tokens(x: torch.Tensor, w_router: torch.Tensor, w_in: torch.Tensor, 
         x = x.contiguous()
     if shared is not None:
         shared = shared.contiguous()
-    L = _lib.lib()
     out = torch.empty((N, D), dtype=x.dtype, device=dev)
     ids = torch.empty((N, top_k), dtype=torch.int32, device=dev)
     probs = torch.empty((N, top_k), dtype=torch.float32, device=dev)
-    scratch = torch.empty(int(L.nsb_moe_few_tokens_scratch_bytes(N, E, top_k, D, F)), dtype=torch.uint8, device=dev)
-    p = _lib.ptr
-    with torch.cuda.device(dev):
-        _lib.check(L.nsb_moe_few_tokens(p(x), x.stride(0), p(w_router), p(w_in), p(w_out), p(shared), p(out), p(ids),
-                                        p(probs), p(scratch), N, E, top_k, D, F, code, _lib.stream_ptr(dev)),
-                   "nsb_moe_few_tokens")
+    scratch = torch.empty(_lib.lib().nsb_moe_few_tokens_scratch_bytes(N, E, top_k, D, F), dtype=torch.uint8, device=dev)
+    at = _lib.address
+    _lib.launch(dev, "nsb_moe_few_tokens", at(x), x.stride(0), at(w_router), at(w_in), at(w_out), at(shared), at(out),
+                at(ids), at(probs), at(scratch), N, E, top_k, D, F, code)
     return (out, ids, probs) if return_routing else out

@@ -27,7 +27,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "nsb_common.cuh"
+#include "nsb_cols.cuh"
 
 namespace nsb {
 namespace {
@@ -55,75 +55,20 @@ struct GatedParams {
   unsigned long long limit_ns;
 };
 
-// Arithmetic on a thread's V columns, two per instruction where V allows (same roundings).
-#define NSB_PAIR(x, i) (*reinterpret_cast<unsigned long long*>(&(x)[i]))
-#define NSB_CPAIR(x, i) (*reinterpret_cast<const unsigned long long*>(&(x)[i]))
-template <int V>
-struct alignas(V >= 2 ? 8 : 4) Cols {
-  float v[V];
-  __device__ __forceinline__ float& operator[](int i) { return v[i]; }
-  __device__ __forceinline__ const float& operator[](int i) const { return v[i]; }
-};
-template <int V>
-__device__ __forceinline__ Cols<V> all(float c) {
-  Cols<V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r[i] = c;
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Cols<V> fma(const Cols<V>& a, const Cols<V>& b, const Cols<V>& c) {
-  Cols<V> r;
-  if constexpr (V % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < V; i += 2)
-      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(NSB_PAIR(r.v, i))
-          : "l"(NSB_CPAIR(a.v, i)), "l"(NSB_CPAIR(b.v, i)), "l"(NSB_CPAIR(c.v, i)));
-  } else {
-    r[0] = fmaf(a[0], b[0], c[0]);
-  }
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Cols<V> mul(const Cols<V>& a, const Cols<V>& b) {
-  Cols<V> r;
-  if constexpr (V % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < V; i += 2)
-      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(NSB_PAIR(r.v, i)) : "l"(NSB_CPAIR(a.v, i)), "l"(NSB_CPAIR(b.v, i)));
-  } else {
-    r[0] = __fmul_rn(a[0], b[0]);
-  }
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Cols<V> add(const Cols<V>& a, const Cols<V>& b) {
-  Cols<V> r;
-  if constexpr (V % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < V; i += 2)
-      asm("add.rn.f32x2 %0, %1, %2;" : "=l"(NSB_PAIR(r.v, i)) : "l"(NSB_CPAIR(a.v, i)), "l"(NSB_CPAIR(b.v, i)));
-  } else {
-    r[0] = __fadd_rn(a[0], b[0]);
-  }
-  return r;
-}
-
 // f = sigmoid(a + b) and m = sigmoid(-(a + b)) from e = exp(-(a + b)): f = 1 / (1 + e), m = e f, neither of them
 // a difference, so both keep their digits however small they are. The exponent is capped where f is 2^-126
 // (e f must not become inf * 0); min.NaN lets a NaN through. `b2` = -b log2(e).
-constexpr float kLog2e = 1.4426950408889634f;
 template <int V>
 __device__ __forceinline__ void gate(const Cols<V>& a, const Cols<V>& b2, Cols<V>& f, Cols<V>& m) {
   Cols<V> q = fma<V>(a, all<V>(-kLog2e), b2), e;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(q[v]) : "f"(q[v]));  // 126
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[v]) : "f"(q[v]));
+    e[v] = ex2(q[v]);
   }
   q = add<V>(e, all<V>(1.0f));
 #pragma unroll
-  for (int v = 0; v < V; ++v) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f[v]) : "f"(q[v]));
+  for (int v = 0; v < V; ++v) f[v] = rcp(q[v]);
   m = mul<V>(e, f);
 }
 __device__ __forceinline__ float gate_bias(float b) { return b * -kLog2e; }
@@ -325,13 +270,6 @@ __device__ __forceinline__ Cols<V> chunk_start(const GatedParams& p, Early<V>& e
   return start;
 }
 
-template <typename T, int V>
-__device__ __forceinline__ Cols<V> widen(const Vec<T, V>& v) {
-  Cols<V> o;
-#pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = Elem<T>::to_f32(v.v[i]);
-  return o;
-}
 // A thread's inputs in shared memory: slot (stream, step) of B bytes = V elements.
 template <typename T, int V, int S>
 struct Stage {
@@ -389,13 +327,6 @@ struct Stage {
     return c;
   }
 };
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> narrow(const Cols<V>& c) {
-  Vec<T, V> o;
-#pragma unroll
-  for (int v = 0; v < V; ++v) o.v[v] = Elem<T>::from_f32(c[v]);
-  return o;
-}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copies_wait_but_last() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }

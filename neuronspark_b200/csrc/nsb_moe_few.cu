@@ -34,6 +34,7 @@ struct MoeParams {
   int* ids;               // [N, K] experts of a token, best first
   float* probs;           // [N, K]
   float* logits;          // [N, E]
+  float* lparts;          // [CTAs of the cluster][N, E] partial logits
   int* used;              // number of experts in use
   int* entries;           // [min(E, N K)][3] expert, first place in `slots`, number of tokens
   int* slots;             // [N K] token * K + j, by expert
@@ -50,26 +51,27 @@ __device__ __forceinline__ Vec<T, 16 / sizeof(T)> zero_chunk() {
   return v;
 }
 // 16 bytes of a row starting at element k, zeros beyond n. VEC: rows are 16-byte aligned and n is a multiple
-// of a chunk. STREAM: read once, so it should not displace the tokens in the first-level cache.
-template <typename T, bool VEC, bool STREAM>
+// of a chunk. STREAM: read once, so it should not displace the tokens in the first-level cache. WHOLE: all of the chunk
+// lies before n.
+template <typename T, bool VEC, bool STREAM, bool WHOLE>
 __device__ __forceinline__ Vec<T, 16 / sizeof(T)> load_chunk(const T* row, int k, int n) {
   constexpr int C = 16 / sizeof(T);
-  Vec<T, C> v = zero_chunk<T>();
+  Vec<T, C> v;
   if constexpr (VEC) {
-    if (row && k < n) {
-      uint4 u;
+    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+    if (WHOLE || k < n) {
       if constexpr (STREAM)
         asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(row + k));
       else
         u = *reinterpret_cast<const uint4*>(row + k);
-      *reinterpret_cast<uint4*>(&v) = u;
     }
+    *reinterpret_cast<uint4*>(&v) = u;
   } else {
-    if (row)
+    v = zero_chunk<T>();
 #pragma unroll
-      for (int i = 0; i < C; ++i)
-        if (k + i < n) v.v[i] = row[k + i];
+    for (int i = 0; i < C; ++i)
+      if (WHOLE || k + i < n) v.v[i] = row[k + i];
   }
   return v;
 }
@@ -107,24 +109,18 @@ __device__ __forceinline__ void mul_chunk(float (&acc)[4], const Vec<T, 8>& lo_r
   mma16(acc, a[2], b[2], a[3], b[3], q[2], q[3], T());
 }
 // fp32 operands: three products of 11-bit terms (the fourth, lo x lo, is below 2^-22)
-template <int C>
-__device__ __forceinline__ void mul_f32(float (&acc)[4], const float* a, const float* b, const float (&w)[C],
-                                        bool w_exact) {
-#pragma unroll
-  for (int i = 0; i < C; i += 2) {
-    uint32_t h[6], l[6];
-    split_tf32(a[i], h[0], l[0]), split_tf32(b[i], h[1], l[1]);
-    split_tf32(a[i + 1], h[2], l[2]), split_tf32(b[i + 1], h[3], l[3]);
-    if (w_exact) h[4] = __float_as_uint(w[i]), h[5] = __float_as_uint(w[i + 1]);
-    else split_tf32(w[i], h[4], l[4]), split_tf32(w[i + 1], h[5], l[5]);
-    mma_tf32(acc, l[0], l[1], l[2], l[3], h[4], h[5]);
-    if (!w_exact) mma_tf32(acc, h[0], h[1], h[2], h[3], l[4], l[5]);
-    mma_tf32(acc, h[0], h[1], h[2], h[3], h[4], h[5]);
-  }
-}
 __device__ __forceinline__ void mul_chunk(float (&acc)[4], const Vec<float, 4>& lo_row, const Vec<float, 4>& hi_row,
                                           const Vec<float, 4>& w) {
-  mul_f32<4>(acc, lo_row.v, hi_row.v, w.v, false);
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    uint32_t h[6], l[6];
+    split_tf32(lo_row.v[i], h[0], l[0]), split_tf32(hi_row.v[i], h[1], l[1]);
+    split_tf32(lo_row.v[i + 1], h[2], l[2]), split_tf32(hi_row.v[i + 1], h[3], l[3]);
+    split_tf32(w.v[i], h[4], l[4]), split_tf32(w.v[i + 1], h[5], l[5]);
+    mma_tf32(acc, l[0], l[1], l[2], l[3], h[4], h[5]);
+    mma_tf32(acc, h[0], h[1], h[2], h[3], l[4], l[5]);
+    mma_tf32(acc, h[0], h[1], h[2], h[3], h[4], h[5]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------ routing
@@ -135,48 +131,87 @@ __device__ __forceinline__ unsigned long long order_key(float v, int index) {
   return ((unsigned long long)s << 32) | (0xffffffffu - (uint32_t)index);
 }
 
-// One cluster of 8 CTAs. A warp takes an expert and four tokens at a time; when all logits are there, the
-// first CTA picks every token's experts (a warp per token) and lists the tokens of every expert.
+// How the cluster's warps share out the logits: tiles of 16 tokens x 8 experts; the blocks of the summation index go
+// round the CTAs, and within a CTA `split` warps take every split-th of its blocks of a tile.
+struct RouteShare {
+  int etiles, tiles, split;
+  __host__ __device__ RouteShare(int N, int E) {
+    etiles = (E + 7) / 8;
+    tiles = (N + 15) / 16 * etiles;
+    split = 1;
+    while (split * 2 * (tiles > 0 ? tiles : 1) <= kRouterThreads / 32) split *= 2;
+  }
+};
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// One cluster of 8 CTAs: partial logits, their sums, every token's choice (a warp per token), and in the first CTA the
+// list of every expert's tokens; a cluster barrier between each. The partial sums are added in a fixed order.
 template <typename T, bool VEC>
 __global__ void __cluster_dims__(kRouterCtas, 1, 1) __launch_bounds__(kRouterThreads) moe_route_kernel(const MoeParams p) {
   constexpr int C = 16 / sizeof(T);
-  __shared__ uint16_t s_ids[kMaxSlots];
-  __shared__ int s_count[kMaxExperts], s_first[kMaxExperts], s_place[kMaxExperts], s_warp[2][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ __align__(16) uint16_t s_ids[kMaxSlots];
+  __shared__ int s_warp[2][32];
+  __shared__ float s_acc[4][kRouterThreads];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x;
+  const int g = lane >> 2, t = lane & 3;
   grid_dependents_may_launch();
+  const RouteShare share(p.N, p.E);
   const T* x = static_cast<const T*>(p.x);
   const T* wr = static_cast<const T*>(p.w_router);
-  const int groups = (p.N + 3) / 4;
-  for (int i = blockIdx.x * (kRouterThreads / 32) + warp; i < p.E * groups; i += kRouterCtas * (kRouterThreads / 32)) {
-    const int e = i % p.E, n0 = i / p.E * 4;
+  const int sw = warp % share.split, parts = kRouterCtas * share.split;
+  float* part = p.lparts + (long long)rank * p.N * p.E;
+  for (int i = warp / share.split; i < share.tiles; i += kRouterThreads / 32 / share.split) {
+    const int n0 = i / share.etiles * 16, e0 = i % share.etiles * 8;
+    // (rows beyond the last stand for tokens and experts that nobody asks for)
+    const T* row_a = x + min(n0 + g, p.N - 1) * p.x_stride;
+    const T* row_b = x + min(n0 + g + 8, p.N - 1) * p.x_stride;
+    const T* row_w = wr + (long long)min(e0 + g, p.E - 1) * p.D;
     float acc[4] = {};
-    for (int k = lane * C; k < p.D; k += 32 * C) {
-      const Vec<T, C> w = load_chunk<T, VEC, false>(wr + (long long)e * p.D, k, p.D);
+#pragma unroll 4
+    for (int k = (rank * share.split + sw) * 4 * C + t * C; k - t * C < p.D; k += parts * 4 * C)
+      mul_chunk(acc, load_chunk<T, VEC, false, false>(row_a, k, p.D), load_chunk<T, VEC, false, false>(row_b, k, p.D),
+                load_chunk<T, VEC, false, false>(row_w, k, p.D));
+    if (share.split > 1) {  // (then every warp has one tile at most)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const Vec<T, C> v = load_chunk<T, VEC, false>(n0 + t < p.N ? x + (n0 + t) * p.x_stride : nullptr, k, p.D);
+      for (int j = 0; j < 4; ++j) s_acc[j][threadIdx.x] = acc[j];
+    }
+    if (share.split == 1)
 #pragma unroll
-        for (int j = 0; j < C; ++j) acc[t] = fmaf(Elem<T>::to_f32(v.v[j]), Elem<T>::to_f32(w.v[j]), acc[t]);
+      for (int j = 0; j < 4; ++j) {
+        const int n = n0 + g + (j >> 1) * 8, e = e0 + 2 * t + (j & 1);
+        if (n < p.N && e < p.E) part[n * p.E + e] = acc[j];
       }
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
-      if (lane == 0 && n0 + t < p.N) p.logits[(n0 + t) * p.E + e] = acc[t];
-    }
   }
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (blockIdx.x != 0) return;
-
-  for (int n = warp; n < p.N; n += kRouterThreads / 32) {
+  if (share.split > 1) {
+    __syncthreads();
+    const int i = warp / share.split, n0 = i / share.etiles * 16, e0 = i % share.etiles * 8;
+    if (sw == 0 && i < share.tiles)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = n0 + g + (j >> 1) * 8, e = e0 + 2 * t + (j & 1);
+        float sum = s_acc[j][threadIdx.x];
+        for (int k = 1; k < share.split; ++k) sum += s_acc[j][threadIdx.x + 32 * k];
+        if (n < p.N && e < p.E) part[n * p.E + e] = sum;
+      }
+  }
+  cluster_barrier();
+  for (int i = rank * kRouterThreads + threadIdx.x; i < p.N * p.E; i += kRouterCtas * kRouterThreads) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kRouterCtas; ++j) sum += __ldcg(p.lparts + (long long)j * p.N * p.E + i);
+    p.logits[i] = sum;
+  }
+  cluster_barrier();
+  for (int n = rank + kRouterCtas * warp; n < p.N; n += kRouterCtas * (kRouterThreads / 32)) {
     uint32_t taken = 0;
     float best = 0.0f, l_j = 0.0f;
     for (int j = 0; j < p.K; ++j) {
       unsigned long long top = 0;
       for (int i = 0; i * 32 + lane < p.E; ++i)
         if (!((taken >> i) & 1u)) {
-          const unsigned long long key = order_key(p.logits[n * p.E + i * 32 + lane], i * 32 + lane);
+          const unsigned long long key = order_key(__ldcg(p.logits + n * p.E + i * 32 + lane), i * 32 + lane);
           top = key > top ? key : top;
         }
 #pragma unroll
@@ -186,13 +221,10 @@ __global__ void __cluster_dims__(kRouterCtas, 1, 1) __launch_bounds__(kRouterThr
       }
       const int e = (int)(0xffffffffu - (uint32_t)top);
       if ((e & 31) == lane) taken |= 1u << (e >> 5);
-      const float l = p.logits[n * p.E + e];
+      const float l = __ldcg(p.logits + n * p.E + e);
       if (j == 0) best = l;
       if (lane == j) l_j = l;
-      if (lane == 0) {
-        p.ids[n * p.K + j] = e;
-        s_ids[n * p.K + j] = (uint16_t)e;
-      }
+      if (lane == 0) p.ids[n * p.K + j] = e;
     }
     const float w = lane < p.K ? expf(l_j - best) : 0.0f;
     float sum = w;
@@ -200,53 +232,61 @@ __global__ void __cluster_dims__(kRouterCtas, 1, 1) __launch_bounds__(kRouterThr
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane < p.K) p.probs[n * p.K + lane] = w / sum;
   }
-  __syncthreads();
+  cluster_barrier();
+  if (rank != 0) return;
+
   // thread e counts expert e's tokens; sums over the threads before it give its place among the experts in
   // use and in the list of slots
   const int e = threadIdx.x, slots = p.N * p.K;
+  for (int i = threadIdx.x; i < kMaxSlots; i += kRouterThreads) s_ids[i] = i < slots ? (uint16_t)__ldcg(p.ids + i) : 0xffffu;
+  __syncthreads();
+  auto visit = [&](auto f) {  // f(slot) for every slot of expert e, in order
+    for (int i = 0; i < slots; i += 8) {
+      const uint4 q = *reinterpret_cast<const uint4*>(s_ids + i);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if ((w[j] & 0xffffu) == (uint32_t)e) f(i + 2 * j);
+        if (w[j] >> 16 == (uint32_t)e) f(i + 2 * j + 1);
+      }
+    }
+  };
   int count = 0;
-  if (e < p.E)
-    for (int i = 0; i < slots; ++i) count += s_ids[i] == e;
-  int before = count, rank = count > 0;
+  if (e < p.E) visit([&](int) { ++count; });
+  int before = count, place = count > 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, before, o), b = __shfl_up_sync(0xffffffffu, rank, o);
-    if (lane >= o) before += a, rank += b;
+    const int a = __shfl_up_sync(0xffffffffu, before, o), b = __shfl_up_sync(0xffffffffu, place, o);
+    if (lane >= o) before += a, place += b;
   }
-  if (lane == 31) s_warp[0][warp] = before, s_warp[1][warp] = rank;
+  if (lane == 31) s_warp[0][warp] = before, s_warp[1][warp] = place;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) before += s_warp[0][w], rank += s_warp[1][w];
-  if (threadIdx.x == kRouterThreads - 1) *p.used = rank;
+  for (int w = 0; w < warp; ++w) before += s_warp[0][w], place += s_warp[1][w];
+  if (threadIdx.x == kRouterThreads - 1) *p.used = place;
   if (count > 0) {
     int at = before - count;
-    p.entries[3 * (rank - 1)] = e;
-    p.entries[3 * (rank - 1) + 1] = at;
-    p.entries[3 * (rank - 1) + 2] = count;
-    for (int i = 0; i < slots; ++i)
-      if (s_ids[i] == e) p.slots[at++] = i;
+    p.entries[3 * (place - 1)] = e;
+    p.entries[3 * (place - 1) + 1] = at;
+    p.entries[3 * (place - 1) + 2] = count;
+    visit([&](int i) { p.slots[at++] = i; });
   }
   for (int i = threadIdx.x; i < p.tiles; i += kRouterThreads) p.done[i] = 0u;
 }
 
 // ------------------------------------------------------------------------------------------ products
 
-// How the warps of a CTA share out a unit: WK of them take every WK-th block of the summation index, 4 / WK units
-// lie side by side. Block: 4 steps of 4 chunks.
+// WK warps of a CTA share a unit, each with every WK-th block of the summation index, and 4 / WK units lie side by side.
+// Block: 4 steps of 4 chunks.
 constexpr int kSteps = 4;
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 
+// A token's hidden values for one chunk, as the down product wants them. 16-bit weights: the hidden value as the sum of
+// two bf16 numbers, off by 2^-16 at most and with fp32's range (rounding it to one number of the weights' type would
+// add an error as large as that of the rounded output itself, and in fp16 it may overflow).
 template <typename T>
-struct ActRow;  // a token's hidden values for one chunk, as the down product wants them
-template <>
-struct ActRow<__nv_bfloat16> {
-  // bf16 weights: the hidden value as the sum of two bf16 numbers, 16 significant bits; rounding it to one would
-  // add an error as large as that of the rounded output itself
+struct ActRow {
   Vec<__nv_bfloat16, 8> hi, lo;
-};
-template <>
-struct ActRow<__half> {  // fp16 weights are exact in 11 bits, and the hidden value may lie outside fp16's range
-  Vec<float, 8> v;
 };
 template <>
 struct ActRow<float> {
@@ -257,45 +297,46 @@ __device__ __forceinline__ void mul_act(float (&acc)[4], const ActRow<__nv_bfloa
   mul_chunk<__nv_bfloat16>(acc, a.lo, b.lo, w);
   mul_chunk<__nv_bfloat16>(acc, a.hi, b.hi, w);
 }
+// An fp16 number is the sum of two bf16 ones exactly: its 8 leading bits and the 3 below them. Of the four products the
+// smallest, lo x lo, is at most 2^-15 of the whole and left out.
 __device__ __forceinline__ void mul_act(float (&acc)[4], const ActRow<__half>& a, const ActRow<__half>& b,
                                         const Vec<__half, 8>& w) {
-  float f[8];
+  Vec<__nv_bfloat16, 8> hi, lo;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = __half2float(w.v[i]);
-  mul_f32<8>(acc, a.v.v, b.v.v, f, true);
+  for (int i = 0; i < 8; i += 2) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w.v[i]));
+    const uint32_t x = __float_as_uint(f.x), y = __float_as_uint(f.y);
+    // (below 256 in size; the minimum takes the NaN that an infinite weight leaves here to a number)
+    const float rx = fminf(f.x - __uint_as_float(x & 0xffff0000u), 256.0f);
+    const float ry = fminf(f.y - __uint_as_float(y & 0xffff0000u), 256.0f);
+    *reinterpret_cast<uint32_t*>(&hi.v[i]) = __byte_perm(x, y, 0x7632);
+    *reinterpret_cast<uint32_t*>(&lo.v[i]) = __byte_perm(__float_as_uint(rx), __float_as_uint(ry), 0x7632);
+  }
+  mul_chunk<__nv_bfloat16>(acc, a.lo, b.lo, hi);
+  mul_chunk<__nv_bfloat16>(acc, a.hi, b.hi, lo);
+  mul_chunk<__nv_bfloat16>(acc, a.hi, b.hi, hi);
 }
 __device__ __forceinline__ void mul_act(float (&acc)[4], const ActRow<float>& a, const ActRow<float>& b,
                                         const Vec<float, 4>& w) {
-  mul_f32<4>(acc, a.v.v, b.v.v, w.v, false);
+  mul_chunk(acc, a.v, b.v, w);
 }
-template <typename T>
-__device__ __forceinline__ ActRow<T> load_act(const void* act, long long slots, int slot, int Fp, int k) {
+template <typename T, bool WHOLE>
+__device__ __forceinline__ ActRow<T> load_act(const char* row, long long second, int k, int Fp) {
   ActRow<T> r;
-  if constexpr (sizeof(T) == 2 && Elem<T>::kDtype == NSB_BF16) {
-    r.hi = r.lo = zero_chunk<T>();
-    if (slot >= 0 && k < Fp) {
-      const T* row = static_cast<const T*>(act) + (long long)slot * Fp + k;
-      r.hi = *reinterpret_cast<const Vec<T, 8>*>(row);
-      r.lo = *reinterpret_cast<const Vec<T, 8>*>(row + slots * Fp);
-    }
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat16* at = reinterpret_cast<const __nv_bfloat16*>(row);
+    r.hi = load_chunk<__nv_bfloat16, true, false, WHOLE>(at, k, Fp);
+    r.lo = load_chunk<__nv_bfloat16, true, false, WHOLE>(at + second, k, Fp);
   } else {
-    constexpr int C = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < C; ++i) r.v.v[i] = 0.0f;
-    if (slot >= 0 && k < Fp) {
-      const float* row = static_cast<const float*>(act) + (long long)slot * Fp + k;
-#pragma unroll
-      for (int i = 0; i < C; i += 4)
-        *reinterpret_cast<Vec<float, 4>*>(&r.v.v[i]) = *reinterpret_cast<const Vec<float, 4>*>(row + i);
-    }
+    r.v = load_chunk<float, true, false, WHOLE>(reinterpret_cast<const float*>(row), k, Fp);
   }
   return r;
 }
 template <typename T>
 __device__ __forceinline__ void store_act(void* act, long long slots, int slot, int Fp, int f, float v) {
-  if constexpr (sizeof(T) == 2 && Elem<T>::kDtype == NSB_BF16) {
-    T* at = static_cast<T*>(act) + (long long)slot * Fp + f;
-    const T hi = __float2bfloat16_rn(v);
+  if constexpr (sizeof(T) == 2) {
+    __nv_bfloat16* at = static_cast<__nv_bfloat16*>(act) + (long long)slot * Fp + f;
+    const __nv_bfloat16 hi = __float2bfloat16_rn(v);
     const float r = v - __bfloat162float(hi);
     at[0] = hi;
     at[slots * Fp] = __float2bfloat16_rn(isfinite(r) ? r : 0.0f);
@@ -318,61 +359,88 @@ __device__ __forceinline__ void add_up(float (&acc)[R], float* buf, int wk, int 
       for (int i = 0; i < R; ++i) acc[i] += buf[i * kThreads + threadIdx.x + 32 * w];
 }
 
-// Unit: 8 hidden values of one expert for all its tokens (8 gate rows and 8 up rows of Win).
-template <typename T, bool VEC, int MT>
-__global__ void __launch_bounds__(kThreads) moe_up_kernel(const MoeParams p, int WK) {
-  constexpr int C = 16 / sizeof(T);
-  __shared__ float buf[MT * 8 * kThreads];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int wk = warp % WK, per_cta = kWarps / WK;
-  grid_dependents_may_launch();
-  grid_dependency_wait();
-  const int per_expert = (p.F + 7) / 8, ctas = (per_expert + per_cta - 1) / per_cta;
-  const int place = blockIdx.x / ctas;
-  if (place >= *p.used) return;
-  const int e = p.entries[3 * place], first = p.entries[3 * place + 1], n = p.entries[3 * place + 2];
-  const int f0 = ((blockIdx.x % ctas) * per_cta + warp / WK) * 8;
-  const int mtiles = (n + 15) / 16;
-  const T* gate_row = nullptr;
-  const T* up_row = nullptr;
-  if (f0 + g < p.F) {
-    gate_row = static_cast<const T*>(p.w_in) + ((long long)e * 2 * p.F + f0 + g) * p.D;
-    up_row = gate_row + (long long)p.F * p.D;
-  }
-  const T* rows[MT][2];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = m * 16 + h * 8 + g;
-      rows[m][h] = i < n ? static_cast<const T*>(p.x) + (p.slots[first + i] / p.K) * p.x_stride : nullptr;
-    }
-  float acc[MT * 8];
-#pragma unroll
-  for (int i = 0; i < MT * 8; ++i) acc[i] = 0.0f;
-  auto part = [&](int i) -> float(&)[4] { return *reinterpret_cast<float(*)[4]>(&acc[4 * i]); };
-  constexpr int kBlock = kSteps * 4 * C;
-  for (int k0 = wk * kBlock; k0 < p.D; k0 += WK * kBlock) {
-    Vec<T, C> wg[kSteps], wu[kSteps];
+// The products of two tiles of 8 weight rows (lane's rows w0 and w1 of n elements) with up to 16 MT tokens:
+// `tokens(whole, m, h, k)` is the lane's chunk at k of its token row h of 16-row tile m, `mul(acc, a, b, w)` the product of
+// a chunk. A warp takes every WK-th block of the summation index; only the last, partial one looks where its row
+// ends. With one tile of tokens, the usual case, the next block's weights are on their way while this one's are
+// multiplied.
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+template <typename T, bool VEC, int MT, typename Tokens, typename Mul>
+__device__ __forceinline__ void weight_products(float (&acc)[MT * 8], const T* w0, const T* w1, int n, int wk, int WK, int mtiles,
+                                                Tokens tokens, Mul mul) {
+  constexpr int C = 16 / sizeof(T), kBlock = kSteps * 4 * C;
+  const int t = threadIdx.x & 3;
+  using Weights = Vec<T, C>[kSteps][2];
+  auto load = [&](auto whole, Weights& w, int k0) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int k = k0 + (s * 4 + t) * C;
-      wg[s] = load_chunk<T, VEC, true>(gate_row, k, p.D);
-      wu[s] = load_chunk<T, VEC, true>(up_row, k, p.D);
+      w[s][0] = load_chunk<T, VEC, true, decltype(whole)::value>(w0, k0 + (s * 4 + t) * C, n);
+      w[s][1] = load_chunk<T, VEC, true, decltype(whole)::value>(w1, k0 + (s * 4 + t) * C, n);
     }
+  };
+  auto multiply = [&](auto whole, Weights& w, int k0) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (m >= mtiles) break;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const int k = k0 + (s * 4 + t) * C;
-        const Vec<T, C> a = load_chunk<T, VEC, false>(rows[m][0], k, p.D);
-        const Vec<T, C> b = load_chunk<T, VEC, false>(rows[m][1], k, p.D);
-        mul_chunk(part(2 * m), a, b, wg[s]);
-        mul_chunk(part(2 * m + 1), a, b, wu[s]);
+        const auto x = tokens(whole, m, 0, k), y = tokens(whole, m, 1, k);
+        mul(*reinterpret_cast<float(*)[4]>(&acc[8 * m]), x, y, w[s][0]);
+        mul(*reinterpret_cast<float(*)[4]>(&acc[8 * m + 4]), x, y, w[s][1]);
       }
     }
+  };
+  const int step = WK * kBlock;
+  int k0 = wk * kBlock;
+  Weights a;
+  if constexpr (MT == 1) {
+    Weights b;
+    if (k0 + kBlock <= n) load(Yes(), a, k0);
+    while (k0 + kBlock <= n) {
+      if (k0 + step + kBlock <= n) load(Yes(), b, k0 + step);
+      multiply(Yes(), a, k0);
+      k0 += step;
+      if (k0 + kBlock > n) break;
+      if (k0 + step + kBlock <= n) load(Yes(), a, k0 + step);
+      multiply(Yes(), b, k0);
+      k0 += step;
+    }
+  } else {
+    for (; k0 + kBlock <= n; k0 += step) {
+      load(Yes(), a, k0);
+      multiply(Yes(), a, k0);
+    }
   }
+  if (k0 < n) {
+    load(No(), a, k0);
+    multiply(No(), a, k0);
+  }
+}
+
+// Unit: 8 hidden values of one expert for all its tokens (8 gate rows and 8 up rows of Win).
+template <typename T, bool VEC, int MT>
+__device__ __forceinline__ void up_unit(const MoeParams& p, int e, int first, int n, int f0, int wk, int WK, float* buf) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  // (rows of weights and tokens beyond the last stand for products that are not kept)
+  const T* gate_row = static_cast<const T*>(p.w_in) + ((long long)e * 2 * p.F + min(f0 + g, p.F - 1)) * p.D;
+  const T* up_row = gate_row + (long long)p.F * p.D;
+  const T* rows[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = m * 16 + h * 8 + g;
+      rows[m][h] = static_cast<const T*>(p.x) + (p.slots[first + min(i, n - 1)] / p.K) * p.x_stride;
+    }
+  float acc[MT * 8];
+#pragma unroll
+  for (int i = 0; i < MT * 8; ++i) acc[i] = 0.0f;
+  weight_products<T, VEC, MT>(
+      acc, gate_row, up_row, p.D, wk, WK, (n + 15) / 16,
+      [&](auto whole, int m, int h, int k) { return load_chunk<T, VEC, false, decltype(whole)::value>(rows[m][h], k, p.D); },
+      [](float (&c)[4], const auto& a, const auto& b, const auto& w) { mul_chunk(c, a, b, w); });
   add_up<MT * 8>(acc, buf, wk, WK);
   if (wk != 0) return;
 #pragma unroll
@@ -382,87 +450,111 @@ __global__ void __launch_bounds__(kThreads) moe_up_kernel(const MoeParams p, int
       const int row = m * 16 + (i >> 1) * 8 + g, f = f0 + 2 * t + (i & 1);
       if (row < n && f < p.Fp) {
         const int slot = p.slots[first + row];
-        const float v = f < p.F ? silu(part(2 * m)[i]) * part(2 * m + 1)[i] * p.probs[slot] : 0.0f;
+        const float v = f < p.F ? silu(acc[8 * m + i]) * acc[8 * m + 4 + i] * p.probs[slot] : 0.0f;
         store_act<T>(p.act, p.N * p.K, slot, p.Fp, f, v);
       }
     }
 }
+template <typename T, bool VEC, int MT>
+__global__ void __launch_bounds__(kThreads, 4) moe_up_kernel(const MoeParams p, int WK) {
+  __shared__ float buf[MT * 8 * kThreads];
+  const int warp = threadIdx.x >> 5, per_cta = kWarps / WK;
+  const int per_expert = (p.F + 7) / 8, ctas = (per_expert + per_cta - 1) / per_cta;
+  const int place = blockIdx.x / ctas, f0 = ((blockIdx.x % ctas) * per_cta + warp / WK) * 8;
+  grid_dependents_may_launch();
+  grid_dependency_wait();
+  if (place >= *p.used) return;
+  const int e = p.entries[3 * place], first = p.entries[3 * place + 1], n = p.entries[3 * place + 2];
+  if constexpr (MT > 1)
+    if (n > 16) {
+      up_unit<T, VEC, MT>(p, e, first, n, f0, warp % WK, WK, buf);
+      return;
+    }
+  up_unit<T, VEC, 1>(p, e, first, n, f0, warp % WK, WK, buf);
+}
 
 // Unit: 16 outputs of one expert for all its tokens. The last unit of an output tile adds up the token's experts.
 template <typename T, bool VEC, int MT>
-__global__ void __launch_bounds__(kThreads) moe_down_kernel(const MoeParams p, int WK) {
-  constexpr int C = 16 / sizeof(T);
-  __shared__ float buf[MT * 8 * kThreads];
-  __shared__ bool s_last;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int wk = warp % WK, per_cta = kWarps / WK;
-  grid_dependency_wait();
-  const int ctas = p.tiles;  // tiles of 16 per_cta outputs
-  const int place = blockIdx.x / ctas, tile = blockIdx.x % ctas, used = *p.used;
-  if (place >= used) return;
-  const int e = p.entries[3 * place], first = p.entries[3 * place + 1], n = p.entries[3 * place + 2];
-  const int d0 = (tile * per_cta + warp / WK) * 16;
-  const int mtiles = (n + 15) / 16;
-  const T* w_row[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    w_row[h] = d0 + 8 * h + g < p.D ? static_cast<const T*>(p.w_out) + ((long long)e * p.D + d0 + 8 * h + g) * p.F : nullptr;
-  int rows[MT][2];
+__device__ __forceinline__ void down_unit(const MoeParams& p, int e, int first, int n, int d0, int wk, int WK, float* buf) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const T* w = static_cast<const T*>(p.w_out) + (long long)e * p.D * p.F;
+  const char* rows[MT][2];
+  const long long second = (long long)p.N * p.K * p.Fp;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int i = m * 16 + h * 8 + g;
-      rows[m][h] = i < n ? p.slots[first + i] : -1;
+      rows[m][h] = static_cast<const char*>(p.act) + (long long)p.slots[first + min(i, n - 1)] * p.Fp * (sizeof(T) == 2 ? 2 : 4);
     }
   float acc[MT * 8];
 #pragma unroll
   for (int i = 0; i < MT * 8; ++i) acc[i] = 0.0f;
-  auto part = [&](int i) -> float(&)[4] { return *reinterpret_cast<float(*)[4]>(&acc[4 * i]); };
-  constexpr int kBlock = kSteps * 4 * C;
-  for (int k0 = wk * kBlock; k0 < p.F; k0 += WK * kBlock) {
-    Vec<T, C> w[kSteps][2];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) w[s][h] = load_chunk<T, VEC, true>(w_row[h], k0 + (s * 4 + t) * C, p.F);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      if (m >= mtiles) break;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int k = k0 + (s * 4 + t) * C;
-        const ActRow<T> a = load_act<T>(p.act, p.N * p.K, rows[m][0], p.Fp, k);
-        const ActRow<T> b = load_act<T>(p.act, p.N * p.K, rows[m][1], p.Fp, k);
-        mul_act(part(2 * m), a, b, w[s][0]);
-        mul_act(part(2 * m + 1), a, b, w[s][1]);
-      }
-    }
-  }
+  weight_products<T, VEC, MT>(
+      acc, w + (long long)min(d0 + g, p.D - 1) * p.F, w + (long long)min(d0 + 8 + g, p.D - 1) * p.F, p.F, wk, WK, (n + 15) / 16,
+      [&](auto whole, int m, int h, int k) { return load_act<T, decltype(whole)::value>(rows[m][h], second, k, p.Fp); },
+      [](float (&c)[4], const auto& a, const auto& b, const auto& q) { mul_act(c, a, b, q); });
   add_up<MT * 8>(acc, buf, wk, WK);
-  if (wk == 0) {
+  if (wk != 0) return;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = m * 16 + ((i >> 1) & 1) * 8 + g, d = d0 + (i >> 2) * 8 + 2 * t + (i & 1);
-        if (row < n && d < p.D) p.part[(long long)p.slots[first + row] * p.D + d] = acc[m * 8 + i];
-      }
-    __threadfence();
-  }
+    for (int i = 0; i < 8; ++i) {
+      const int row = m * 16 + ((i >> 1) & 1) * 8 + g, d = d0 + (i >> 2) * 8 + 2 * t + (i & 1);
+      if (row < n && d < p.D) p.part[(long long)p.slots[first + row] * p.D + d] = acc[m * 8 + i];
+    }
+}
+template <typename T, bool VEC, int MT>
+__global__ void __launch_bounds__(kThreads, 4) moe_down_kernel(const MoeParams p, int WK) {
+  __shared__ float buf[MT * 8 * kThreads];
+  __shared__ bool s_last;
+  const int warp = threadIdx.x >> 5, per_cta = kWarps / WK;
+  const int place = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;  // tiles of 16 per_cta outputs
+  const int d0 = (tile * per_cta + warp / WK) * 16;
+  grid_dependency_wait();
+  const int used = *p.used;
+  if (place >= used) return;
+  const int e = p.entries[3 * place], first = p.entries[3 * place + 1], n = p.entries[3 * place + 2];
+  bool wide = false;
+  if constexpr (MT > 1) wide = n > 16;
+  if (wide) down_unit<T, VEC, MT>(p, e, first, n, d0, warp % WK, WK, buf);
+  else down_unit<T, VEC, 1>(p, e, first, n, d0, warp % WK, WK, buf);
+  __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) s_last = atomicAdd(p.done + tile, 1u) + 1u == (unsigned)used;
   __syncthreads();
   if (!s_last) return;
   __threadfence();
   const int width = 16 * per_cta, base = tile * width;
-  for (int i = threadIdx.x; i < p.N * width; i += kThreads) {
-    const int tok = i / width, d = base + i % width;
-    if (d >= p.D) continue;
-    float sum = p.shared ? Elem<T>::to_f32(static_cast<const T*>(p.shared)[(long long)tok * p.D + d]) : 0.0f;
-    for (int j = 0; j < p.K; ++j) sum += __ldcg(p.part + ((long long)tok * p.K + j) * p.D + d);
-    static_cast<T*>(p.out)[(long long)tok * p.D + d] = Elem<T>::from_f32(sum);
-  }
+  auto add_experts = [&](auto quad) {  // four outputs per thread and turn, or one where rows do not divide by four
+    constexpr int Q = decltype(quad)::value ? 4 : 1;
+    const int across = width / Q;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.N * across; i += kThreads) {
+      const int tok = i / across, d = base + i % across * Q;
+      if (d >= p.D) continue;
+      const long long at = (long long)tok * p.D + d;
+      float sum[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) sum[q] = p.shared ? Elem<T>::to_f32(static_cast<const T*>(p.shared)[at + q]) : 0.0f;
+      const float* part = p.part + (long long)tok * p.K * p.D + d;
+#pragma unroll 4
+      for (int j = 0; j < p.K; ++j, part += p.D) {
+        float v[Q];
+        if constexpr (Q == 4) {
+          const float4 f = __ldcg(reinterpret_cast<const float4*>(part));
+          v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        } else {
+          v[0] = __ldcg(part);
+        }
+#pragma unroll
+        for (int q = 0; q < Q; ++q) sum[q] += v[q];
+      }
+#pragma unroll
+      for (int q = 0; q < Q; ++q) static_cast<T*>(p.out)[at + q] = Elem<T>::from_f32(sum[q]);
+    }
+  };
+  if (p.D % 4 == 0) add_experts(Yes()); else add_experts(No());
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -472,13 +564,14 @@ bool fits(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a =
 long long up16(long long n) { return (n + 15) / 16 * 16; }
 
 struct Layout {  // of the workspace, in bytes
-  long long logits, used, entries, slots, done, act, part, bytes;
+  long long logits, lparts, used, entries, slots, done, act, part, bytes;
 };
 Layout layout(long long N, long long E, long long K, long long D, long long F) {
   const long long S = N * K, Fp = (F + 7) / 8 * 8;
   Layout l;
   l.logits = 0;
-  l.used = up16(N * E * 4);
+  l.lparts = up16(N * E * 4);
+  l.used = l.lparts + up16(N * E * 4 * kRouterCtas);
   l.entries = l.used + 16;
   l.slots = l.entries + up16(12 * std::min(E, S));
   l.done = l.slots + up16(4 * S);
@@ -564,6 +657,7 @@ extern "C" int nsb_moe_few_tokens(const void* x, int64_t x_stride, const void* w
   char* base = static_cast<char*>(scratch);
   p.ids = ids, p.probs = probs;
   p.logits = reinterpret_cast<float*>(base + l.logits);
+  p.lparts = reinterpret_cast<float*>(base + l.lparts);
   p.used = reinterpret_cast<int*>(base + l.used);
   p.entries = reinterpret_cast<int*>(base + l.entries);
   p.slots = reinterpret_cast<int*>(base + l.slots);

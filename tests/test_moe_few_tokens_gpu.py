@@ -1,9 +1,9 @@
 """The expert layer for a few tokens against the same layer in 64 bits.
 
-Bounds. A logit sums D/32 products per lane and 5 shuffles, each rounding at most 2^-24 of the sum of absolute
-values. A tensor-core product adds 16 (fp32 operands: 8, three times) summands to its fp32 accumulator; taking
-2^-22 of the sum of absolute values for each such addition covers truncation and the alignment inside it. Hidden
-values keep 16 bits with bf16 weights (two bf16 terms: 2^-17 is left), 2^-21 otherwise. p is off by twice the
+Bounds. A tensor-core product adds 16 (fp32 operands: 8, three times) summands to its fp32 accumulator; taking
+2^-22 of the sum of absolute values for each such addition covers truncation and the alignment inside it. A logit is
+such sums of at most every eighth block each, added up in fp32, and fp32 operands lose 2^-20 of each product. Hidden
+values keep 2^-16 with 16-bit weights, 2^-21 otherwise. p is off by twice the
 logits' error, and silu's slope is at most 1.1. The output adds half a step of its type. Which experts are taken is
 checked against the 64-bit logits up to their error, and the values with the experts that were taken."""
 import pytest
@@ -31,7 +31,8 @@ def check(x, wr, wi, wo, k, shared, got):
     assert out.shape == (N, D) and out.dtype == dt and ids.dtype == torch.int32 and p.dtype == torch.float32
     X, WR = x.double(), wr.double()
     logits = X @ WR.T
-    e_l = ((D / 32 + 8) * 2.0 ** -24 * (X.abs() @ WR.abs().T)).amax(1, keepdim=True)
+    per = (2.0 ** -22 * 3 / 8, 2.0 ** -20) if dt == torch.float32 else (2.0 ** -22 / 16, 0.0)
+    e_l = ((D / 8 * per[0] + per[1] + 16 * 2.0 ** -22) * (X.abs() @ WR.abs().T)).amax(1, keepdim=True)
     ids = ids.long()
     taken = torch.zeros(N, E, dtype=torch.bool, device=DEV).scatter_(1, ids, True)
     assert (taken.sum(1) == k).all()  # distinct
@@ -45,8 +46,11 @@ def check(x, wr, wi, wo, k, shared, got):
     value = torch.zeros(N, D, dtype=torch.float64, device=DEV) if shared is None else shared.double()
     err = (k + 2) * 2.0 ** -24 * value.abs()
     add = 2.0 ** -22 * (3 / 8 if dt == torch.float32 else 1 / 16)
-    left = 2.0 ** -17 if dt == torch.bfloat16 else 2.0 ** -20
-    add2 = 2.0 ** -22 * (2 / 16 if dt == torch.bfloat16 else 3 / 8)
+    # 16-bit weights: the hidden value in two bf16 terms, the second at most 2^-8 of it and itself rounded by 2^-8; fp16
+    # weights are exact in two bf16 terms, the second (what lies behind 8 bits) below 2^-7, and the product of both second
+    # terms, 2^-8 x 2^-7, is left out: 2^-16 + 2^-15
+    left = {torch.bfloat16: 2.0 ** -16, torch.float16: 1.5 * 2.0 ** -15, torch.float32: 2.0 ** -20}[dt]
+    add2 = 2.0 ** -22 * {torch.bfloat16: 2 / 16, torch.float16: 3 / 16, torch.float32: 3 / 8}[dt]
     for n in range(N):
         for j in range(k):
             W, O = wi[ids[n, j]].double(), wo[ids[n, j]].double()

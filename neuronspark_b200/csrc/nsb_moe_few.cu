@@ -211,7 +211,7 @@ __global__ void __cluster_dims__(kRouterCtas, 1, 1) __launch_bounds__(kRouterThr
       unsigned long long top = 0;
       for (int i = 0; i * 32 + lane < p.E; ++i)
         if (!((taken >> i) & 1u)) {
-          const unsigned long long key = order_key(__ldcg(p.logits + n * p.E + i * 32 + lane), i * 32 + lane);
+          const unsigned long long key = order_key(p.logits[n * p.E + i * 32 + lane], i * 32 + lane);
           top = key > top ? key : top;
         }
 #pragma unroll
@@ -221,7 +221,7 @@ __global__ void __cluster_dims__(kRouterCtas, 1, 1) __launch_bounds__(kRouterThr
       }
       const int e = (int)(0xffffffffu - (uint32_t)top);
       if ((e & 31) == lane) taken |= 1u << (e >> 5);
-      const float l = __ldcg(p.logits + n * p.E + e);
+      const float l = p.logits[n * p.E + e];
       if (j == 0) best = l;
       if (lane == j) l_j = l;
       if (lane == 0) p.ids[n * p.K + j] = e;
@@ -276,8 +276,12 @@ __global__ void __cluster_dims__(kRouterCtas, 1, 1) __launch_bounds__(kRouterThr
 // ------------------------------------------------------------------------------------------ products
 
 // WK warps of a CTA share a unit, each with every WK-th block of the summation index, and 4 / WK units lie side by side.
-// Block: 4 steps of 4 chunks.
-constexpr int kSteps = 4;
+// Block: some steps of 4 chunks.
+// Steps of a block and CTAs per SM (registers): a warp of the up product has 4 x 1 KB of weights and the tokens' chunks for
+// them on their way; the down product, whose tokens come as two terms, 1 x 1 KB, and more warps. Measured with others:
+// (4, 3 CTAs; 1, 5 CTAs) 156 us for 16 tokens and 303 us for 64, (4, 3; 2, 4) 160 and 310, (2, 5; 2, 4) 167 and 314, without
+// the tokens ahead (4, 4; 4, 4) 185 and 352.
+constexpr int kUpSteps = 4, kDownSteps = 1;
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 
@@ -363,59 +367,82 @@ __device__ __forceinline__ void add_up(float (&acc)[R], float* buf, int wk, int 
 // `tokens(whole, m, h, k)` is the lane's chunk at k of its token row h of 16-row tile m, `mul(acc, a, b, w)` the product of
 // a chunk. A warp takes every WK-th block of the summation index; only the last, partial one looks where its row
 // ends. With one tile of tokens, the usual case, the next block's weights are on their way while this one's are
-// multiplied.
+// multiplied, and the first block's while `prepare` looks up where the tokens lie.
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
-template <typename T, bool VEC, int MT, typename Tokens, typename Mul>
+template <typename T, bool VEC, int MT, int KS, typename Prepare, typename Tokens, typename Mul>
 __device__ __forceinline__ void weight_products(float (&acc)[MT * 8], const T* w0, const T* w1, int n, int wk, int WK, int mtiles,
-                                                Tokens tokens, Mul mul) {
-  constexpr int C = 16 / sizeof(T), kBlock = kSteps * 4 * C;
+                                                Prepare prepare, Tokens tokens, Mul mul) {
+  constexpr int C = 16 / sizeof(T), kBlock = KS * 4 * C;
   const int t = threadIdx.x & 3;
-  using Weights = Vec<T, C>[kSteps][2];
-  auto load = [&](auto whole, Weights& w, int k0) {
+  using Row = decltype(tokens(Yes(), 0, 0, 0));
+  struct Block {
+    Vec<T, C> w[KS][2];
+    Row x[KS][2];
+  };
+  auto at = [&](int k0, int s) { return k0 + (s * 4 + t) * C; };
+  auto load_weights = [&](auto whole, Block& b, int k0) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      w[s][0] = load_chunk<T, VEC, true, decltype(whole)::value>(w0, k0 + (s * 4 + t) * C, n);
-      w[s][1] = load_chunk<T, VEC, true, decltype(whole)::value>(w1, k0 + (s * 4 + t) * C, n);
+    for (int s = 0; s < KS; ++s) {
+      b.w[s][0] = load_chunk<T, VEC, true, decltype(whole)::value>(w0, at(k0, s), n);
+      b.w[s][1] = load_chunk<T, VEC, true, decltype(whole)::value>(w1, at(k0, s), n);
     }
   };
-  auto multiply = [&](auto whole, Weights& w, int k0) {
+  auto load_tokens = [&](auto whole, Block& b, int m, int k0) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      if (m >= mtiles) break;
+    for (int s = 0; s < KS; ++s) {
+      b.x[s][0] = tokens(whole, m, 0, at(k0, s));
+      b.x[s][1] = tokens(whole, m, 1, at(k0, s));
+    }
+  };
+  auto multiply = [&](Block& b, int m) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int k = k0 + (s * 4 + t) * C;
-        const auto x = tokens(whole, m, 0, k), y = tokens(whole, m, 1, k);
-        mul(*reinterpret_cast<float(*)[4]>(&acc[8 * m]), x, y, w[s][0]);
-        mul(*reinterpret_cast<float(*)[4]>(&acc[8 * m + 4]), x, y, w[s][1]);
-      }
+    for (int s = 0; s < KS; ++s) {
+      mul(*reinterpret_cast<float(*)[4]>(&acc[8 * m]), b.x[s][0], b.x[s][1], b.w[s][0]);
+      mul(*reinterpret_cast<float(*)[4]>(&acc[8 * m + 4]), b.x[s][0], b.x[s][1], b.w[s][1]);
     }
   };
   const int step = WK * kBlock;
   int k0 = wk * kBlock;
-  Weights a;
+  Block a;
   if constexpr (MT == 1) {
-    Weights b;
-    if (k0 + kBlock <= n) load(Yes(), a, k0);
+    Block b;
+    if (k0 + kBlock <= n) load_weights(Yes(), a, k0);
+    prepare();
+    if (k0 + kBlock <= n) load_tokens(Yes(), a, 0, k0);
+    auto next = [&](Block& from, Block& to) {
+      if (k0 + step + kBlock <= n) {
+        load_weights(Yes(), to, k0 + step);
+        load_tokens(Yes(), to, 0, k0 + step);
+      }
+      multiply(from, 0);
+      k0 += step;
+    };
     while (k0 + kBlock <= n) {
-      if (k0 + step + kBlock <= n) load(Yes(), b, k0 + step);
-      multiply(Yes(), a, k0);
-      k0 += step;
+      next(a, b);
       if (k0 + kBlock > n) break;
-      if (k0 + step + kBlock <= n) load(Yes(), a, k0 + step);
-      multiply(Yes(), b, k0);
-      k0 += step;
+      next(b, a);
     }
   } else {
+    prepare();
     for (; k0 + kBlock <= n; k0 += step) {
-      load(Yes(), a, k0);
-      multiply(Yes(), a, k0);
+      load_weights(Yes(), a, k0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m >= mtiles) break;
+        load_tokens(Yes(), a, m, k0);
+        multiply(a, m);
+      }
     }
   }
   if (k0 < n) {
-    load(No(), a, k0);
-    multiply(No(), a, k0);
+    load_weights(No(), a, k0);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (m >= mtiles) break;
+      load_tokens(No(), a, m, k0);
+      multiply(a, m);
+    }
   }
 }
 
@@ -427,18 +454,18 @@ __device__ __forceinline__ void up_unit(const MoeParams& p, int e, int first, in
   const T* gate_row = static_cast<const T*>(p.w_in) + ((long long)e * 2 * p.F + min(f0 + g, p.F - 1)) * p.D;
   const T* up_row = gate_row + (long long)p.F * p.D;
   const T* rows[MT][2];
+  auto prepare = [&] {
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = m * 16 + h * 8 + g;
-      rows[m][h] = static_cast<const T*>(p.x) + (p.slots[first + min(i, n - 1)] / p.K) * p.x_stride;
-    }
+      for (int h = 0; h < 2; ++h)
+        rows[m][h] = static_cast<const T*>(p.x) + (p.slots[first + min(m * 16 + h * 8 + g, n - 1)] / p.K) * p.x_stride;
+  };
   float acc[MT * 8];
 #pragma unroll
   for (int i = 0; i < MT * 8; ++i) acc[i] = 0.0f;
-  weight_products<T, VEC, MT>(
-      acc, gate_row, up_row, p.D, wk, WK, (n + 15) / 16,
+  weight_products<T, VEC, MT, kUpSteps>(
+      acc, gate_row, up_row, p.D, wk, WK, (n + 15) / 16, prepare,
       [&](auto whole, int m, int h, int k) { return load_chunk<T, VEC, false, decltype(whole)::value>(rows[m][h], k, p.D); },
       [](float (&c)[4], const auto& a, const auto& b, const auto& w) { mul_chunk(c, a, b, w); });
   add_up<MT * 8>(acc, buf, wk, WK);
@@ -456,15 +483,15 @@ __device__ __forceinline__ void up_unit(const MoeParams& p, int e, int first, in
     }
 }
 template <typename T, bool VEC, int MT>
-__global__ void __launch_bounds__(kThreads, 4) moe_up_kernel(const MoeParams p, int WK) {
+__global__ void __launch_bounds__(kThreads, 3) moe_up_kernel(const MoeParams p, int WK) {
   __shared__ float buf[MT * 8 * kThreads];
   const int warp = threadIdx.x >> 5, per_cta = kWarps / WK;
   const int per_expert = (p.F + 7) / 8, ctas = (per_expert + per_cta - 1) / per_cta;
   const int place = blockIdx.x / ctas, f0 = ((blockIdx.x % ctas) * per_cta + warp / WK) * 8;
   grid_dependents_may_launch();
   grid_dependency_wait();
-  if (place >= *p.used) return;
-  const int e = p.entries[3 * place], first = p.entries[3 * place + 1], n = p.entries[3 * place + 2];
+  const int used = *p.used, e = p.entries[3 * place], first = p.entries[3 * place + 1], n = p.entries[3 * place + 2];
+  if (place >= used) return;  // (there is an entry, of no meaning, for every CTA)
   if constexpr (MT > 1)
     if (n > 16) {
       up_unit<T, VEC, MT>(p, e, first, n, f0, warp % WK, WK, buf);
@@ -480,18 +507,19 @@ __device__ __forceinline__ void down_unit(const MoeParams& p, int e, int first, 
   const T* w = static_cast<const T*>(p.w_out) + (long long)e * p.D * p.F;
   const char* rows[MT][2];
   const long long second = (long long)p.N * p.K * p.Fp;
+  auto prepare = [&] {
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = m * 16 + h * 8 + g;
-      rows[m][h] = static_cast<const char*>(p.act) + (long long)p.slots[first + min(i, n - 1)] * p.Fp * (sizeof(T) == 2 ? 2 : 4);
-    }
+      for (int h = 0; h < 2; ++h)
+        rows[m][h] = static_cast<const char*>(p.act) +
+                     (long long)p.slots[first + min(m * 16 + h * 8 + g, n - 1)] * p.Fp * (sizeof(T) == 2 ? 2 : 4);
+  };
   float acc[MT * 8];
 #pragma unroll
   for (int i = 0; i < MT * 8; ++i) acc[i] = 0.0f;
-  weight_products<T, VEC, MT>(
-      acc, w + (long long)min(d0 + g, p.D - 1) * p.F, w + (long long)min(d0 + 8 + g, p.D - 1) * p.F, p.F, wk, WK, (n + 15) / 16,
+  weight_products<T, VEC, MT, kDownSteps>(
+      acc, w + (long long)min(d0 + g, p.D - 1) * p.F, w + (long long)min(d0 + 8 + g, p.D - 1) * p.F, p.F, wk, WK, (n + 15) / 16, prepare,
       [&](auto whole, int m, int h, int k) { return load_act<T, decltype(whole)::value>(rows[m][h], second, k, p.Fp); },
       [](float (&c)[4], const auto& a, const auto& b, const auto& q) { mul_act(c, a, b, q); });
   add_up<MT * 8>(acc, buf, wk, WK);
@@ -505,16 +533,15 @@ __device__ __forceinline__ void down_unit(const MoeParams& p, int e, int first, 
     }
 }
 template <typename T, bool VEC, int MT>
-__global__ void __launch_bounds__(kThreads, 4) moe_down_kernel(const MoeParams p, int WK) {
+__global__ void __launch_bounds__(kThreads, 5) moe_down_kernel(const MoeParams p, int WK) {
   __shared__ float buf[MT * 8 * kThreads];
   __shared__ bool s_last;
   const int warp = threadIdx.x >> 5, per_cta = kWarps / WK;
   const int place = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;  // tiles of 16 per_cta outputs
   const int d0 = (tile * per_cta + warp / WK) * 16;
   grid_dependency_wait();
-  const int used = *p.used;
+  const int used = *p.used, e = p.entries[3 * place], first = p.entries[3 * place + 1], n = p.entries[3 * place + 2];
   if (place >= used) return;
-  const int e = p.entries[3 * place], first = p.entries[3 * place + 1], n = p.entries[3 * place + 2];
   bool wide = false;
   if constexpr (MT > 1) wide = n > 16;
   if (wide) down_unit<T, VEC, MT>(p, e, first, n, d0, warp % WK, WK, buf);

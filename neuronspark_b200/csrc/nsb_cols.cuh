@@ -102,6 +102,15 @@ __device__ __forceinline__ Vec<T, V> narrow(const Cols<V>& c) {
   return o;
 }
 
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_if(bool on, const T* p) {
+  Vec<T, V> v;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v.v[i] = Elem<T>::zero();
+  if (on) v = *reinterpret_cast<const Vec<T, V>*>(p);
+  return v;
+}
+
 __device__ __forceinline__ float ex2(float q) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(q));

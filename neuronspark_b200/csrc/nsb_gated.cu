@@ -24,6 +24,9 @@
 //
 // CTAs stay and take tile after tile: the next tile's inputs are copied to shared memory (by the thread that
 // will use them, so that nothing needs a barrier) while this one is worked on.
+//
+// Long forwards with packed sequences or few columns go another way: one launch finds the maps of all chunks, one
+// takes the state through them, and one works on the chunks from known states, reading the inputs a second time.
 #include <algorithm>
 #include <atomic>
 
@@ -53,6 +56,7 @@ struct GatedParams {
   uint32_t* ticket;
   uint2* maps;                      // [nchunks][cols] (P, H)
   uint32_t* states;                 // [nchunks / g][cols]
+  float* starts;                    // [nchunks][cols]: the states before the chunks, of three launches
   uint32_t* err;
   unsigned long long limit_ns;
 };
@@ -357,7 +361,7 @@ struct Tile {
 // A CTA's tiles. CHAIN: tickets, drawn by one thread and passed on at the barrier that every tile has. Where chunks
 // pass maps, the next one is drawn when a tile is begun, not earlier: tiles are then begun nearly in the order of
 // their numbers, and none that others wait for lies behind another tile in its own CTA (two drawn at the start
-// put every second one there: 450 us instead of 130 for 32768 x 768 bf16). With g = 1 only the block's own previous
+// put every second one there, 3.5 times the time). With g = 1 only the block's own previous
 // chunk matters, long done, so tickets are drawn, and inputs copied, one tile further ahead. Without CHAIN there is
 // one chunk, and every CTA has its share of its blocks.
 template <bool CHAIN>
@@ -433,9 +437,9 @@ __device__ __forceinline__ void put_state(const GatedParams& p, float* to, const
 }
 // An empty sequence ends in the state that it starts from (and hands back what it is handed).
 template <int V>
-__device__ __forceinline__ void empty_sequences(const GatedParams& p, const float* from, float* to, int col, int wt_idx) {
+__device__ __forceinline__ void empty_sequences(const GatedParams& p, const float* from, float* to, int col, int first, int step) {
   if (to)
-    for (int q = wt_idx; q < p.S_seqs; q += p.wt)
+    for (int q = first; q < p.S_seqs; q += step)
       if (__ldg(p.cu + q + 1) <= __ldg(p.cu + q))
 #pragma unroll
         for (int v = 0; v < V; ++v)
@@ -551,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const GatedParam
     };
     if (plain) run(No()); else run(Yes());
     if constexpr (PACKED)
-      if (tile.pos == 0 && on) empty_sequences<V>(p, p.h0, p.h_last, col, wt_idx);
+      if (tile.pos == 0 && on) empty_sequences<V>(p, p.h0, p.h_last, col, wt_idx, p.wt);
     tile = next;
     next = drawn;
     bias = next_bias;
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 3) gated_bwd_kernel(const GatedParam
     if (plain) run(No()); else run(Yes());
     s_db[threadIdx.x] = db;
     if constexpr (PACKED)
-      if (chunk == 0 && on) empty_sequences<V>(p, p.dh_last, p.d_h0, col, wt_idx);
+      if (chunk == 0 && on) empty_sequences<V>(p, p.dh_last, p.d_h0, col, wt_idx, p.wt);
     before = tile;
     tile = next;
     next = drawn;
@@ -722,6 +726,219 @@ __global__ void __launch_bounds__(kThreads, 3) gated_bwd_kernel(const GatedParam
   }
   __syncthreads();
   if (before.pos >= 0) bias_sum(before);
+}
+
+// ---- long forwards: three launches instead of one
+//
+// Handing states from chunk to chunk inside a launch costs a round of waiting per round of resident tiles, and with
+// packed sequences the search for those of a tile's rows lies on that path. Three launches read the inputs twice instead: the chunks' maps, their
+// composition along time, then every chunk from its starting state. A warp has 64 steps of 32 V columns to itself, one
+// after the other, so nothing is kept, exchanged or waited for inside a launch.
+
+// row_kinds of a whole chunk at once: the search for the sequences of its rows runs once, a row per lane and turn
+struct ChunkRows {
+  unsigned long long in, first, last;
+  int seq[2];  // lane l: of rows l and l + 32
+  template <int S>
+  __device__ __forceinline__ Rows block(int i, int lane) const {
+    Rows r;
+    const uint32_t mask = (1u << S) - 1u;
+    r.in = (uint32_t)(in >> (i * S)) & mask;
+    r.first = (uint32_t)(first >> (i * S)) & mask;
+    r.last = (uint32_t)(last >> (i * S)) & mask;
+    r.seq = __shfl_sync(0xffffffffu, i * S < 32 ? seq[0] : seq[1], (i * S + lane) & 31);
+    return r;
+  }
+};
+template <bool PACKED>
+__device__ __forceinline__ ChunkRows chunk_rows(const GatedParams& p, int t0, int lane) {
+  ChunkRows c = {0ull, 0ull, 0ull, {0, 0}};
+  if constexpr (PACKED) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = t0 + 32 * h + lane;
+      int lo = 0, hi = t < p.T ? p.S_seqs : 0;  // sequences that end at or before row t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(p.cu + mid + 1) <= t) lo = mid + 1; else hi = mid;
+      }
+      bool in = t < p.T && lo < p.S_seqs, first = false, last = false;
+      if (in) {
+        const int begin = __ldg(p.cu + lo), end = __ldg(p.cu + lo + 1);
+        in = begin <= t;
+        first = begin == t;
+        last = in && end == t + 1;
+      }
+      c.seq[h] = in ? lo : 0;
+      c.in |= (unsigned long long)__ballot_sync(0xffffffffu, in) << (32 * h);
+      c.first |= (unsigned long long)__ballot_sync(0xffffffffu, first) << (32 * h);
+      c.last |= (unsigned long long)__ballot_sync(0xffffffffu, last) << (32 * h);
+    }
+  } else {
+    const int left = p.T - t0;
+    c.in = left >= 64 ? ~0ull : (1ull << left) - 1ull;
+    c.first = t0 == 0 ? 1ull : 0ull;
+    c.last = left <= 64 ? 1ull << (left - 1) : 0ull;
+  }
+  return c;
+}
+static_assert(kCkptRows == 64, "");
+
+// Rows that a warp requests together: 2 KB of each input, or 16 rows. (A second set of registers to request the next rows
+// into spilled and was slower: 44 us instead of 37 for the last launch of 32768 x 768 bf16.)
+template <typename T, int V>
+constexpr int kRowsInFlight = V * sizeof(T) == 8 ? 8 : 16;
+
+// The map (P, H) of every chunk.
+template <typename T, int V, bool PACKED>
+__global__ void __launch_bounds__(kThreads, 3) gated_maps_kernel(const GatedParams p) {
+  constexpr int S = kRowsInFlight<T, V>;
+  const int lane = threadIdx.x & 31;
+  const long long id = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  grid_dependents_may_launch();
+  const int chunk = (int)(id / p.nb), col = (int)(id - (long long)chunk * p.nb) * (32 * V) + lane * V;
+  if (chunk >= p.nchunks) return;
+  const bool on = col < p.cols;
+  const T* raw = static_cast<const T*>(p.raw) + (on ? input_at(p, col, p.raw_st, p.raw_sb, 0) : 0);
+  const T* x = static_cast<const T*>(p.x) + (on ? input_at(p, col, p.x_st, p.x_sb, 0) : 0);
+  const Cols<V> bias = mul<V>(load_bias<V>(p, col, on), all<V>(-kLog2e));
+  MapV<V> m = {all<V>(1.0f), all<V>(0.0f)};
+  const ChunkRows kinds = chunk_rows<PACKED>(p, chunk * kCkptRows, lane);
+  for (int i = 0; i < kCkptRows / S; ++i) {
+    const int t0 = chunk * kCkptRows + i * S;
+    const T* raw_t = raw + t0 * p.raw_st;
+    const T* x_t = x + t0 * p.x_st;
+    Vec<T, V> vr[S], vx[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s, raw_t += p.raw_st, x_t += p.x_st) {
+      const bool in = on && t0 + s < p.T;
+      vr[s] = load_if<T, V>(in, raw_t);
+      vx[s] = load_if<T, V>(in, x_t);
+    }
+    const Rows rows = kinds.block<S>(i, lane);
+    auto steps = [&](auto special) {
+      constexpr bool kSpecial = decltype(special)::value;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if constexpr (kSpecial)
+          if ((rows.first >> s) & 1u) m = {all<V>(kCut), state_at<PACKED, V>(p, p.h0, rows, s, col, on)};
+        Cols<V> f, u;
+        gate<V>(widen<T, V>(vr[s]), bias, f, u);
+        m.P = mul<V>(m.P, f);
+        m.H = fma<V>(f, m.H, mul<V>(u, widen<T, V>(vx[s])));
+      }
+    };
+    if (rows.plain(S)) steps(No()); else steps(Yes());
+  }
+  if (on)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      p.maps[(long long)chunk * p.cols + col + v] = make_uint2(__float_as_uint(m.P[v]), __float_as_uint(m.H[v]));
+}
+
+// starts[i] = the state after the maps 0 .. i - 1, from zero. A CTA has 32 columns; warp w composes the w-th part of the chunks,
+// takes the parts before its own from shared memory, and goes through its chunks again.
+template <bool PACKED>
+__global__ void __launch_bounds__(1024) gated_chain_kernel(const GatedParams p) {
+  __shared__ MapV<1> parts[32][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  grid_dependents_may_launch();
+  grid_dependency_wait();
+  const int per = (p.nchunks + 31) / 32, a = min(w * per, p.nchunks), b = min(a + per, p.nchunks);
+  const bool on = col < p.cols;
+  const uint2* maps = p.maps + col;
+  constexpr int kBatch = 16;  // maps on their way together
+  uint2 q[kBatch];
+  auto load = [&](int from) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      q[k] = on && from + k < b ? __ldcg(maps + (long long)(from + k) * p.cols) : make_uint2(0x3f800000u, 0u);
+  };
+  auto map_of = [&](int k) {
+    MapV<1> m;
+    m.P[0] = __uint_as_float(q[k].x), m.H[0] = __uint_as_float(q[k].y);
+    return m;
+  };
+  MapV<1> m = {all<1>(1.0f), all<1>(0.0f)};
+  for (int i = a; i < b; i += kBatch) {
+    load(i);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const MapV<1> t = map_of(k);
+      then_map<PACKED, 1>(m, t.P, t.H);
+    }
+  }
+  parts[w][lane] = m;
+  __syncthreads();
+  Cols<1> h = all<1>(0.0f);
+#pragma unroll 4
+  for (int i = 0; i < w; ++i) h = apply_map<PACKED, 1>(parts[i][lane].P, parts[i][lane].H, h);
+  for (int i = a; i < b; i += kBatch) {
+    if (per > kBatch) load(i);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (i + k < b) {
+        const MapV<1> t = map_of(k);
+        if (on) p.starts[(long long)(i + k) * p.cols + col] = h[0];
+        h = apply_map<PACKED, 1>(t.P, t.H, h);
+      }
+  }
+}
+
+// Every chunk from its starting state, the last chunks first: they are the ones the cache still holds.
+template <typename T, int V, bool PACKED>
+__global__ void __launch_bounds__(kThreads, 3) gated_apply_kernel(const GatedParams p) {
+  constexpr int S = kRowsInFlight<T, V>;
+  const int lane = threadIdx.x & 31;
+  const long long id = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int back = (int)(id / p.nb), chunk = p.nchunks - 1 - back, col = (int)(id - (long long)back * p.nb) * (32 * V) + lane * V;
+  if (chunk < 0) return;
+  const bool on = col < p.cols;
+  const T* raw = static_cast<const T*>(p.raw) + (on ? input_at(p, col, p.raw_st, p.raw_sb, 0) : 0);
+  const T* x = static_cast<const T*>(p.x) + (on ? input_at(p, col, p.x_st, p.x_sb, 0) : 0);
+  T* y = static_cast<T*>(p.y) + col;
+  const Cols<V> bias = mul<V>(load_bias<V>(p, col, on), all<V>(-kLog2e));
+  Cols<V> h;
+  const ChunkRows kinds = chunk_rows<PACKED>(p, chunk * kCkptRows, lane);
+  for (int i = 0; i < kCkptRows / S; ++i) {
+    const int t0 = chunk * kCkptRows + i * S;
+    const T* raw_t = raw + t0 * p.raw_st;
+    const T* x_t = x + t0 * p.x_st;
+    T* y_t = y + (long long)t0 * p.cols;
+    Vec<T, V> vr[S], vx[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s, raw_t += p.raw_st, x_t += p.x_st) {
+      const bool in = on && t0 + s < p.T;
+      vr[s] = load_if<T, V>(in, raw_t);
+      vx[s] = load_if<T, V>(in, x_t);
+    }
+    const Rows rows = kinds.block<S>(i, lane);
+    if (i == 0) {
+      grid_dependency_wait();
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = on ? __ldcg(p.starts + (long long)chunk * p.cols + col + v) : 0.0f;
+    }
+    auto steps = [&](auto special) {
+      constexpr bool kSpecial = decltype(special)::value;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if constexpr (kSpecial)
+          if ((rows.first >> s) & 1u) h = state_at<PACKED, V>(p, p.h0, rows, s, col, on);
+        Cols<V> f, m;
+        gate<V>(widen<T, V>(vr[s]), bias, f, m);
+        h = fma<V>(f, h, mul<V>(m, widen<T, V>(vx[s])));
+        if (on && (!kSpecial || t0 + s < p.T))
+          *reinterpret_cast<Vec<T, V>*>(y_t) =
+              narrow<T, V>(!kSpecial || ((rows.in >> s) & 1u) ? h : all<V>(0.0f));
+        if constexpr (kSpecial)
+          if ((rows.last >> s) & 1u) put_state<PACKED, V>(p, p.h_last, rows, s, col, on, h);
+        y_t += p.cols;
+      }
+    };
+    if (rows.plain(S)) steps(No()); else steps(Yes());
+  }
+  if constexpr (PACKED)
+    if (chunk == 0 && on) empty_sequences<V>(p, p.h0, p.h_last, col, 0, 1);
 }
 
 // d_bias[d] = sum over rows of part[row][d], in 64 bits, in a fixed order: thread (i, j) of a CTA takes rows
@@ -798,12 +1015,13 @@ static_assert(kBwdSteps * kWarps == kCkptRows && kFwdSteps * kWarps >= kCkptRows
 bool ok_dtype(int d) { return d == NSB_F32 || d == NSB_BF16 || d == NSB_F16; }
 bool fits(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// scratch: [ticket, 3 words of padding][states][maps], filled with 0xff by one memset
+// Scratch of a launch that hands over: [ticket, 3 words of padding][states][maps], filled with 0xff by one memset. Of three
+// launches: [maps][starting states].
 long long scratch_words(long long T, long long cols) {
   const long long chunks = bwd_chunks(T);
   if (chunks <= 1) return 0;
-  // whatever g the plan takes: all chunks' maps, or all chunks' states
-  return 4 + ((chunks / 32 + 1) * cols + 3) / 4 * 4 + 2 * chunks * cols;
+  // whatever the plan takes: all chunks' maps and all states
+  return 4 + (3 * chunks * cols + cols + 3) / 4 * 4;
 }
 
 template <typename T, int V, bool BACKWARD, bool PACKED, bool CHAIN>
@@ -824,6 +1042,39 @@ int start_kernel(const GatedParams& p, int ctas, int device, cudaStream_t st) {
   return NSB_OK;
 }
 
+// Three launches read the inputs twice and cost some 25 us of their own, but in none does a chunk wait for another. They are
+// taken for packed sequences (whose search lies on the path of the hand-over) from 40 MB of inputs, else from 64 MB and
+// where there are few columns for the steps. Forward in us, three launches and one, inputs not in any cache: packed
+// 8192 x 768 bf16 50 and 37, 24000 x 768 63 and 79, 32768 x 768 70 and 105, 32768 x 6144 401 and 582, 20011 x 1001 fp16 74 and
+// 145; not packed 16384 x 768 bf16 52 and 43, 32768 x 768 67 and 76, 65536 x 768 fp32 174 and 206, 20011 x 1001 fp16 71 and
+// 101, 16384 x 4096 bf16 153 and 137, 32768 x 6144 384 and 356. The backward's three launches came out within 8% either
+// way of its one, and were dropped.
+bool three_launches(long long T, long long cols, size_t es, bool packed) {
+  const double bytes = 2.0 * (double)T * (double)cols * (double)es;
+  return packed ? bytes >= 40e6 : bytes >= 64e6 && T / 16 >= cols;
+}
+
+template <typename T, int V, bool PACKED>
+int launch_maps(GatedParams p, cudaStream_t st) {
+  p.nb = (int)((p.cols + 32LL * V - 1) / (32 * V));
+  const long long warps = (long long)p.nb * p.nchunks;
+  gated_maps_kernel<T, V, PACKED><<<(unsigned)((warps + kWarps - 1) / kWarps), kThreads, 0, st>>>(p);
+  NSB_CUDA_TRY(cudaGetLastError(), "launch gated_maps_kernel");
+  NSB_CUDA_TRY(launch_dependent(gated_chain_kernel<PACKED>, dim3((unsigned)((p.cols + 31) / 32)), dim3(1024), 0, st, p),
+               "launch gated_chain_kernel");
+  NSB_CUDA_TRY(launch_dependent(gated_apply_kernel<T, V, PACKED>, dim3((unsigned)((warps + kWarps - 1) / kWarps)), dim3(kThreads), 0, st, p),
+               "launch gated_apply_kernel");
+  return NSB_OK;
+}
+
+void set_bias_division(GatedParams& p) {
+  if (p.D <= 1) return;
+  int l = 0;  // division by multiplication (Granlund and Montgomery 1994): m = floor(2^(31 + l) / D) + 1, l = ceil(log2 D)
+  while ((1LL << l) < p.D) ++l;
+  p.d_magic = (uint32_t)((1ull << (31 + l)) / (uint64_t)p.D + 1);
+  p.d_shift = l - 1;
+}
+
 template <typename T, bool BACKWARD>
 int launch_gated(GatedParams p, uint32_t* scratch, cudaStream_t st) {
   DeviceInfo dev;
@@ -840,20 +1091,32 @@ int launch_gated(GatedParams p, uint32_t* scratch, cudaStream_t st) {
       ok = ok && fits(q, a);
     return ok;
   };
+  const bool packed = p.cu != nullptr;
+  const long long chunks = bwd_chunks(p.T);
+  if (!BACKWARD && chunks > 2 && three_launches(p.T, p.cols, sizeof(T), packed)) {
+    if (!scratch || !fits(scratch, 16)) return NSB_ERR_INVALID_ARG;
+    p.nchunks = (int)chunks;
+    set_bias_division(p);
+    p.maps = reinterpret_cast<uint2*>(scratch);
+    p.starts = p.ckpt ? p.ckpt : reinterpret_cast<float*>(scratch + 2 * chunks * p.cols);
+    // 8 bytes of a row per lane, fewer if the chunks then do not give every SM 8 warps
+    int V = 8 / (int)sizeof(T);
+    while (V > 1 && (!all_fit(V) || p.cols <= 16 * V || (p.cols + 32LL * V - 1) / (32 * V) * chunks < 8LL * dev.sm_count)) V /= 2;
+#define NSB_GO_V(V_) (packed ? launch_maps<T, V_, true>(p, st) : launch_maps<T, V_, false>(p, st))
+    if constexpr (sizeof(T) == 2)
+      if (V == 4) return NSB_GO_V(4);
+    return V == 2 ? NSB_GO_V(2) : NSB_GO_V(1);
+#undef NSB_GO_V
+  }
   int V = 4 / (int)sizeof(T);
   while (V > 1 && (!all_fit(V) || p.cols <= 16 * V)) V /= 2;
   const int ctas = dev.sm_count * (BACKWARD ? 3 : 2);
   const GatedPlan q = plan_gated(p.T, p.cols, V, BACKWARD ? kBwdSteps : kFwdSteps, ctas);
   p.nb = q.nb, p.nchunks = q.nchunks, p.g = q.g, p.wt = q.wt;
   while (1 << p.g_log2 < p.g) ++p.g_log2;
-  if (p.D > 1) {  // division by multiplication (Granlund and Montgomery 1994): m = floor(2^(31 + l) / D) + 1, l = ceil(log2 D)
-    int l = 0;
-    while ((1LL << l) < p.D) ++l;
-    p.d_magic = (uint32_t)((1ull << (31 + l)) / (uint64_t)p.D + 1);
-    p.d_shift = l - 1;
-  }
+  set_bias_division(p);
   if ((long long)q.nb * q.nchunks > 0x7fffffffLL - 2 * ctas) return NSB_ERR_TOO_LARGE;
-  const bool chain = q.nchunks > 1, packed = p.cu != nullptr;
+  const bool chain = q.nchunks > 1;
   if (chain) {
     if (!scratch || !fits(scratch, 16)) return NSB_ERR_INVALID_ARG;
     const long long nstates = (q.nchunks / q.g + 1LL) * p.cols;

@@ -79,15 +79,6 @@ __device__ __forceinline__ Cols<V> load_affine(const float* p, int c, float othe
   for (int i = 0; i < V; ++i) o[i] = p ? __ldg(p + c + i) : other;
   return o;
 }
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_if(bool on, const T* p) {
-  Vec<T, V> v;
-#pragma unroll
-  for (int i = 0; i < V; ++i) v.v[i] = Elem<T>::zero();
-  if (on) v = *reinterpret_cast<const Vec<T, V>*>(p);
-  return v;
-}
-
 // Sums of U values over the `team` consecutive threads that share a group; every thread gets them. SHUF: a
 // power of two of at most 32 threads, which then lie in one warp.
 template <int U, bool SHUF>

@@ -163,6 +163,36 @@ def test_packed_long_and_int32():
     compare(got, reference(v["raw"], v["x"], v["h0"], v["bias"], cu, v["dy"], v["dh"]), torch.bfloat16)
 
 
+# 42 to 77 MB of inputs: the forward goes over them twice, in three launches (by 4, 2 and 1 columns of 16 bits, 2 and 1 of 32)
+@pytest.mark.parametrize("packed,dtype,T,D", [(True, torch.bfloat16, 14001, 800), (True, torch.float16, 11003, 998),
+                                              (True, torch.float16, 11003, 1001), (True, torch.float32, 8100, 650),
+                                              (False, torch.bfloat16, 24000, 800), (False, torch.float16, 20011, 1001),
+                                              (False, torch.float32, 13000, 651)])
+def test_long_forwards(packed, dtype, T, D):
+    cu = [0, 1, 3000, 3000, 7001, T - 70, T - 70, T - 10] if packed else None  # (empty ones, and rows behind the last)
+    v = make((T, D), dtype, 59, seqs=len(cu) - 1 if packed else None)
+    if packed:
+        v["x"][5000, 1] = v["raw"][5000, 2] = float("nan")  # one sequence's own
+    cut = torch.tensor(cu, device=DEV) if packed else None
+    with torch.no_grad():
+        y, h_last = gr.gated_linear_recurrence(v["raw"], v["x"], v["h0"], v["bias"], cu_seqlens=cut)
+        again = gr.gated_linear_recurrence(v["raw"], v["x"], v["h0"], v["bias"], cu_seqlens=cut)
+        bare, _ = gr.gated_linear_recurrence(v["raw"], v["x"], cu_seqlens=cut)
+    want = reference(v["raw"], v["x"], v["h0"], v["bias"], cu)
+    close(y, want["y"], dtype, "y")
+    close(h_last, want["h_last"], torch.float32, "h_last")
+    assert torch.equal(y.nan_to_num(7.0), again[0].nan_to_num(7.0)) and torch.equal(h_last.nan_to_num(7.0), again[1].nan_to_num(7.0))
+    close(bare, reference(v["raw"], v["x"], None, None, cu)["y"], dtype, "y without a state or bias")
+
+
+def test_gradients_of_a_long_forward():
+    """The backward starts its chunks from the states that the forward's second launch found; batch-major inputs."""
+    T, B, D = 24000, 2, 400
+    v = make((T, B, D), torch.bfloat16, 61)
+    v = {n: t.transpose(0, 1).contiguous().transpose(0, 1) if n in ("raw", "x", "dy") else t for n, t in v.items()}
+    compare(run(v), reference(v["raw"], v["x"], v["h0"], v["bias"], None, v["dy"], v["dh"]), torch.bfloat16)
+
+
 def test_packed_rows_are_the_sequences_alone():
     """Bit for bit where the chunks lie alike; the state of a sequence never reaches its neighbour."""
     v = make((128, 64), torch.float32, 13, seqs=2)

@@ -84,6 +84,8 @@ class GatedLinearRecurrence(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dh_last):
+        if torch.is_grad_enabled():  # (create_graph=True)
+            raise NSBError("gated_linear_recurrence has no second derivatives")
         a, v, h0, bias, cu, ckpt = ctx.saved_tensors
         T, B, D = _sizes(v)
         dev, dt, L, at = a.device, a.dtype, _lib.lib(), _lib.address

@@ -53,6 +53,8 @@ class GroupNormAct(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_out):
+        if torch.is_grad_enabled():  # (create_graph=True)
+            raise NSBError("group_norm_act has no second derivatives")
         x, w, b, stats = ctx.saved_tensors
         N, L, C, G, act = ctx.sizes
         dev, lib, at = x.device, _lib.lib(), _lib.address

@@ -386,3 +386,11 @@ def test_a_call_after_a_timeout_is_refused():
         nsb.set_wait_limit_ns()
         assert nsb.device_error_word() != 0
     gr.gated_linear_recurrence(v["raw"], v["x"])
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(4, 6, device=DEV, requires_grad=True)
+    y = gr.gated_linear_recurrence(x, x)[0]
+    with pytest.raises(nsb.NSBError, match="second derivatives"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    torch.autograd.grad(y.sum(), x)

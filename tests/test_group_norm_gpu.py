@@ -286,3 +286,11 @@ def test_a_layer_of_all_three(dtype):
     gn.group_norm_act(y.reshape(T * B, D), heads, leaves[2], leaves[3]).float().square().sum().backward()
     assert all(t.grad is not None and torch.isfinite(t.grad).all() and (t.grad != 0).any() for t in leaves)
     assert nsb.device_error_word() == 0
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(4, 6, device=DEV, requires_grad=True)
+    y = gn.group_norm_act(x, 2)
+    with pytest.raises(nsb.NSBError, match="second derivatives"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    torch.autograd.grad(y.sum(), x)

@@ -731,9 +731,10 @@ __global__ void __launch_bounds__(kThreads, 3) gated_bwd_kernel(const GatedParam
 // ---- long forwards: three launches instead of one
 //
 // Handing states from chunk to chunk inside a launch costs a round of waiting per round of resident tiles, and with
-// packed sequences the search for those of a tile's rows lies on that path. Three launches read the inputs twice instead: the chunks' maps, their
-// composition along time, then every chunk from its starting state. A warp has 64 steps of 32 V columns to itself, one
-// after the other, so nothing is kept, exchanged or waited for inside a launch.
+// packed sequences the search for those of a tile's rows lies on that path. Three launches read the inputs twice
+// instead: the chunks' maps, their composition along time, then every chunk from its starting state. A warp has 64 steps
+// of 32 V columns to itself, one after the other, so nothing is kept, exchanged or waited for inside a launch. 32768 x 768
+// bf16: 32 + 6 + 38 us at 0.5 instructions per cycle and scheduler and 41-44% of DRAM's rate, bound by neither alone.
 
 // row_kinds of a whole chunk at once: the search for the sequences of its rows runs once, a row per lane and turn
 struct ChunkRows {

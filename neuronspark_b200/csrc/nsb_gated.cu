@@ -733,8 +733,9 @@ __global__ void __launch_bounds__(kThreads, 3) gated_bwd_kernel(const GatedParam
 // Handing states from chunk to chunk inside a launch costs a round of waiting per round of resident tiles, and with
 // packed sequences the search for those of a tile's rows lies on that path. Three launches read the inputs twice
 // instead: the chunks' maps, their composition along time, then every chunk from its starting state. A warp has 64 steps
-// of 32 V columns to itself, one after the other, so nothing is kept, exchanged or waited for inside a launch. 32768 x 768
-// bf16: 32 + 6 + 38 us at 0.5 instructions per cycle and scheduler and 41-44% of DRAM's rate, bound by neither alone.
+// of 32 V columns to itself, one after the other, so nothing is kept, exchanged or waited for inside a launch. Blocks whose
+// rows and columns are all there load without conditions (32 + 38 us before, for 32768 x 768 bf16). Now 28 + 6 + 33 us, 3.6 and
+// 4.6 TB/s, at half an instruction per cycle and scheduler: bound by neither alone.
 
 // row_kinds of a whole chunk at once: the search for the sequences of its rows runs once, a row per lane and turn
 struct ChunkRows {
@@ -799,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 3) gated_maps_kernel(const GatedPara
   grid_dependents_may_launch();
   const int chunk = (int)(id / p.nb), col = (int)(id - (long long)chunk * p.nb) * (32 * V) + lane * V;
   if (chunk >= p.nchunks) return;
-  const bool on = col < p.cols;
+  const bool on = col < p.cols, whole = col - lane * V + 32 * V <= p.cols;  // (cols below 2^31 - 2^8)
   const T* raw = static_cast<const T*>(p.raw) + (on ? input_at(p, col, p.raw_st, p.raw_sb, 0) : 0);
   const T* x = static_cast<const T*>(p.x) + (on ? input_at(p, col, p.x_st, p.x_sb, 0) : 0);
   const Cols<V> bias = mul<V>(load_bias<V>(p, col, on), all<V>(-kLog2e));
@@ -810,11 +811,19 @@ __global__ void __launch_bounds__(kThreads, 3) gated_maps_kernel(const GatedPara
     const T* raw_t = raw + t0 * p.raw_st;
     const T* x_t = x + t0 * p.x_st;
     Vec<T, V> vr[S], vx[S];
+    if (whole && t0 + S <= p.T) {
 #pragma unroll
-    for (int s = 0; s < S; ++s, raw_t += p.raw_st, x_t += p.x_st) {
-      const bool in = on && t0 + s < p.T;
-      vr[s] = load_if<T, V>(in, raw_t);
-      vx[s] = load_if<T, V>(in, x_t);
+      for (int s = 0; s < S; ++s, raw_t += p.raw_st, x_t += p.x_st) {
+        vr[s] = *reinterpret_cast<const Vec<T, V>*>(raw_t);
+        vx[s] = *reinterpret_cast<const Vec<T, V>*>(x_t);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; ++s, raw_t += p.raw_st, x_t += p.x_st) {
+        const bool in = on && t0 + s < p.T;
+        vr[s] = load_if<T, V>(in, raw_t);
+        vx[s] = load_if<T, V>(in, x_t);
+      }
     }
     const Rows rows = kinds.block<S>(i, lane);
     auto steps = [&](auto special) {
@@ -894,7 +903,7 @@ __global__ void __launch_bounds__(kThreads, 3) gated_apply_kernel(const GatedPar
   const long long id = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int back = (int)(id / p.nb), chunk = p.nchunks - 1 - back, col = (int)(id - (long long)back * p.nb) * (32 * V) + lane * V;
   if (chunk < 0) return;
-  const bool on = col < p.cols;
+  const bool on = col < p.cols, whole = col - lane * V + 32 * V <= p.cols;  // (cols below 2^31 - 2^8)
   const T* raw = static_cast<const T*>(p.raw) + (on ? input_at(p, col, p.raw_st, p.raw_sb, 0) : 0);
   const T* x = static_cast<const T*>(p.x) + (on ? input_at(p, col, p.x_st, p.x_sb, 0) : 0);
   T* y = static_cast<T*>(p.y) + col;
@@ -907,11 +916,19 @@ __global__ void __launch_bounds__(kThreads, 3) gated_apply_kernel(const GatedPar
     const T* x_t = x + t0 * p.x_st;
     T* y_t = y + (long long)t0 * p.cols;
     Vec<T, V> vr[S], vx[S];
+    if (whole && t0 + S <= p.T) {
 #pragma unroll
-    for (int s = 0; s < S; ++s, raw_t += p.raw_st, x_t += p.x_st) {
-      const bool in = on && t0 + s < p.T;
-      vr[s] = load_if<T, V>(in, raw_t);
-      vx[s] = load_if<T, V>(in, x_t);
+      for (int s = 0; s < S; ++s, raw_t += p.raw_st, x_t += p.x_st) {
+        vr[s] = *reinterpret_cast<const Vec<T, V>*>(raw_t);
+        vx[s] = *reinterpret_cast<const Vec<T, V>*>(x_t);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; ++s, raw_t += p.raw_st, x_t += p.x_st) {
+        const bool in = on && t0 + s < p.T;
+        vr[s] = load_if<T, V>(in, raw_t);
+        vx[s] = load_if<T, V>(in, x_t);
+      }
     }
     const Rows rows = kinds.block<S>(i, lane);
     if (i == 0) {
@@ -1046,7 +1063,7 @@ int start_kernel(const GatedParams& p, int ctas, int device, cudaStream_t st) {
 // Three launches read the inputs twice and cost some 25 us of their own, but in none does a chunk wait for another. They are
 // taken for packed sequences (whose search lies on the path of the hand-over) from 40 MB of inputs, else from 64 MB and
 // where there are few columns for the steps. Forward in us, three launches and one, inputs not in any cache: packed
-// 8192 x 768 bf16 50 and 37, 24000 x 768 63 and 79, 32768 x 768 70 and 105, 32768 x 6144 401 and 582, 20011 x 1001 fp16 74 and
+// 8192 x 768 bf16 50 and 37, 24000 x 768 63 and 79, 32768 x 768 66 and 105, 32768 x 6144 401 and 582, 20011 x 1001 fp16 70 and
 // 145; not packed 16384 x 768 bf16 52 and 43, 32768 x 768 67 and 76, 65536 x 768 fp32 174 and 206, 20011 x 1001 fp16 71 and
 // 101, 16384 x 4096 bf16 153 and 137, 32768 x 6144 384 and 356. The backward's three launches came out within 8% either
 // way of its one, and were dropped.

@@ -1060,13 +1060,13 @@ int start_kernel(const GatedParams& p, int ctas, int device, cudaStream_t st) {
   return NSB_OK;
 }
 
-// Three launches read the inputs twice and cost some 25 us of their own, but in none does a chunk wait for another. They are
-// taken for packed sequences (whose search lies on the path of the hand-over) from 40 MB of inputs, else from 64 MB and
-// where there are few columns for the steps. Forward in us, three launches and one, inputs not in any cache: packed
-// 8192 x 768 bf16 50 and 37, 24000 x 768 63 and 79, 32768 x 768 66 and 105, 32768 x 6144 401 and 582, 20011 x 1001 fp16 70 and
-// 145; not packed 16384 x 768 bf16 52 and 43, 32768 x 768 67 and 76, 65536 x 768 fp32 174 and 206, 20011 x 1001 fp16 71 and
-// 101, 16384 x 4096 bf16 153 and 137, 32768 x 6144 384 and 356. The backward's three launches came out within 8% either
-// way of its one, and were dropped.
+// Three launches read the inputs twice and cost some 25 us of their own, but in none does a chunk wait for another. They
+// are taken for packed sequences (whose search lies on the path of the hand-over) from 40 MB of inputs, else from 64 MB
+// and where there are few columns for the steps. Forward in us, three launches and one, inputs not in any cache: packed
+// 16384 x 768 bf16 53 and 61, 24000 x 768 53 and 79, 32768 x 768 61 and 105, 32768 x 6144 338 and 582, 20011 x 1001 fp16 70
+// and 145; not packed 16384 x 768 bf16 44 and 43, 32768 x 768 59 and 76, 65536 x 768 fp32 171 and 206, 20011 x 1001 fp16
+// 64 and 101, 16384 x 4096 bf16 130 and 137, 2048 x 49152 204 and 155, 512 x 393216 487 and 304. The backward's three
+// launches came out within 8% either way of its one, and were dropped.
 bool three_launches(long long T, long long cols, size_t es, bool packed) {
   const double bytes = 2.0 * (double)T * (double)cols * (double)es;
   return packed ? bytes >= 40e6 : bytes >= 64e6 && T / 16 >= cols;

@@ -98,7 +98,7 @@ __device__ __forceinline__ void split_tf32(float v, uint32_t& hi, uint32_t& lo) 
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(isfinite(r) ? r : 0.0f));
 }
 
-// acc += (token rows g and g + 8) x (weight row g) over one chunk per lane, inputs as they are
+// acc += (token rows g and g + 8) x (weight row g) over one chunk per lane, inputs as they are (from zero: see add_chunk)
 template <typename T>
 __device__ __forceinline__ void mul_chunk(float (&acc)[4], const Vec<T, 8>& lo_row, const Vec<T, 8>& hi_row,
                                           const Vec<T, 8>& w) {
@@ -121,6 +121,15 @@ __device__ __forceinline__ void mul_chunk(float (&acc)[4], const Vec<float, 4>& 
     mma_tf32(acc, h[0], h[1], h[2], h[3], l[4], l[5]);
     mma_tf32(acc, h[0], h[1], h[2], h[3], h[4], h[5]);
   }
+}
+
+// The tensor core rounds what it adds to an accumulator toward zero, so one that lived for a whole row would shrink by up to
+// a unit in the last place per product: outputs 2.1e-5 off in fp32 for 64 tokens, 4096 x 1792, where the sum to the nearest
+// is 2e-7 off. So a chunk's product starts from zero, and chunks are added up in fp32 to the nearest (920 -> 1001 us there; no
+// time in bf16).
+__device__ __forceinline__ void add_chunk(float (&acc)[4], const float (&part)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] += part[i];
 }
 
 // ------------------------------------------------------------------------------------------ routing
@@ -170,9 +179,12 @@ __global__ void __cluster_dims__(kRouterCtas, 1, 1) __launch_bounds__(kRouterThr
     const T* row_w = wr + (long long)min(e0 + g, p.E - 1) * p.D;
     float acc[4] = {};
 #pragma unroll 4
-    for (int k = (rank * share.split + sw) * 4 * C + t * C; k - t * C < p.D; k += parts * 4 * C)
-      mul_chunk(acc, load_chunk<T, VEC, false, false>(row_a, k, p.D), load_chunk<T, VEC, false, false>(row_b, k, p.D),
+    for (int k = (rank * share.split + sw) * 4 * C + t * C; k - t * C < p.D; k += parts * 4 * C) {
+      float part_acc[4] = {};
+      mul_chunk(part_acc, load_chunk<T, VEC, false, false>(row_a, k, p.D), load_chunk<T, VEC, false, false>(row_b, k, p.D),
                 load_chunk<T, VEC, false, false>(row_w, k, p.D));
+      add_chunk(acc, part_acc);
+    }
     if (share.split > 1) {  // (then every warp has one tile at most)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s_acc[j][threadIdx.x] = acc[j];
@@ -398,8 +410,11 @@ __device__ __forceinline__ void weight_products(float (&acc)[MT * 8], const T* w
   auto multiply = [&](Block& b, int m) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      mul(*reinterpret_cast<float(*)[4]>(&acc[8 * m]), b.x[s][0], b.x[s][1], b.w[s][0]);
-      mul(*reinterpret_cast<float(*)[4]>(&acc[8 * m + 4]), b.x[s][0], b.x[s][1], b.w[s][1]);
+      float part[2][4] = {};
+      mul(part[0], b.x[s][0], b.x[s][1], b.w[s][0]);
+      mul(part[1], b.x[s][0], b.x[s][1], b.w[s][1]);
+      add_chunk(*reinterpret_cast<float(*)[4]>(&acc[8 * m]), part[0]);
+      add_chunk(*reinterpret_cast<float(*)[4]>(&acc[8 * m + 4]), part[1]);
     }
   };
   const int step = WK * kBlock;

@@ -232,3 +232,23 @@ def test_no_gradients():
         mk.moe_few_tokens(x, wr, wi, wo, 2)
     with torch.no_grad():
         mk.moe_few_tokens(x, wr, wi, wo, 2)
+
+
+def test_long_sums_of_one_sign():
+    """fp32, 32768 positive products a sum: rounding toward zero would lose some 1e-4 of each. Four warps share a row, so a warp
+    adds 32768 / 16 / 4 = 512 chunks, each to the nearest: 512 / 2 half units in the last place (the partial sum is half of
+    the whole on average), 2^-20 of each product and 6 products of a chunk at 2^-22."""
+    D, F = 32768, 8
+    g = torch.Generator(device=DEV).manual_seed(15)
+    x, w_in = (0.5 + torch.rand(s, generator=g, device=DEV) for s in ((2, D), (1, 2 * F, D)))
+    w_in /= D
+    w_out = torch.zeros(1, D, F, device=DEV)
+    w_out[0, :F] = torch.eye(F, device=DEV)
+    out = mk.moe_few_tokens(x, torch.zeros(1, D, device=DEV), w_in, w_out, 1)[:, :F]
+    u = (x.double()[:, None] * w_in.double()).sum(-1)
+    gate, up = u[:, :F], u[:, F:]
+    e = 2.0 ** -20 + 6 * 2.0 ** -22 + (512 / 2 + 8) * 2.0 ** -24
+    s = gate * torch.sigmoid(gate)
+    # the down product: 2^-20 of its one summand, and the sigmoid's, the activation's and p's roundings
+    bound = 1.1 * e * gate * up + (s + 1.1 * e * gate) * e * up + (2.0 ** -20 + 24 * 2.0 ** -24) * s * up
+    assert ((out.double() - s * up).abs() <= bound).all()

@@ -751,7 +751,8 @@ int nsb_gated_recurrence_step(const void* raw, int64_t raw_stride_b, const void*
  * 0..F-1 = Wg, F..2F-1 = Wu; w_out [E, D, F]; shared [N, D] or NULL; out [N, D]; all in
  * `dtype`. ids [N, K] int32 and probs [N, K] fp32: each token's experts, best first, and p.
  * N <= 64, K <= 16, K <= E <= 1024, D and F <= 2^20. Products accumulate in fp32; hidden
- * values keep 2^-16 relative or better between the two products.
+ * values keep 2^-22 relative or better between the two products, fp32 operands 2^-20 of a
+ * product.
  * scratch: nsb_moe_few_tokens_scratch_bytes bytes, 16-byte aligned; one per call in flight.
  */
 int64_t nsb_moe_few_tokens_scratch_bytes(int64_t N, int64_t E, int64_t K, int64_t D, int64_t F);

@@ -39,7 +39,7 @@ struct MoeParams {
   int* entries;           // [min(E, N K)][3] expert, first place in `slots`, number of tokens
   int* slots;             // [N K] token * K + j, by expert
   unsigned int* done;     // [tiles] units of the down product that have finished
-  void* act;              // [N K, Fp] hidden values times p: bf16 as two terms, otherwise fp32
+  void* act;              // hidden values times p, [terms][N K, Fp]: bf16 three bf16 terms, fp16 two tf32 ones, fp32 one
   float* part;            // [N K, D] down products
 };
 
@@ -290,19 +290,30 @@ __global__ void __cluster_dims__(kRouterCtas, 1, 1) __launch_bounds__(kRouterThr
 // WK warps of a CTA share a unit, each with every WK-th block of the summation index, and 4 / WK units lie side by side.
 // Block: some steps of 4 chunks.
 // Steps of a block and CTAs per SM (registers): a warp of the up product has 4 x 1 KB of weights and the tokens' chunks for
-// them on their way; the down product, whose tokens come as two terms, 1 x 1 KB, and more warps. Measured with others:
-// (4, 3 CTAs; 1, 5 CTAs) 156 us for 16 tokens and 303 us for 64, (4, 3; 2, 4) 160 and 310, (2, 5; 2, 4) 167 and 314, without
-// the tokens ahead (4, 4; 4, 4) 185 and 352.
+// them on their way; the down product, whose tokens come as two or three terms, 1 x 1 KB, and more warps. Measured with others, by
+// steps and CTAs: the up product, with two terms in both, (4, 3) 156 us for 16 tokens in fp16 and 303 us for 64 in bf16, (2, 5) 167 and
+// 314 beside (2, 4) below; the down product (1, 5) 208 (it spills) and 316, (1, 4) 157 and 324, (1, 3) 174 and 352, (2, 3) 208 and 336.
 constexpr int kUpSteps = 4, kDownSteps = 1;
+template <typename T>
+constexpr int kDownCtas = Elem<T>::kDtype == NSB_F16 ? 4 : 5;
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 
-// A token's hidden values for one chunk, as the down product wants them. 16-bit weights: the hidden value as the sum of
-// two bf16 numbers, off by 2^-16 at most and with fp32's range (rounding it to one number of the weights' type would
-// add an error as large as that of the rounded output itself, and in fp16 it may overflow).
+// A token's hidden values for one chunk, as the down product wants them: with fp32's range (in fp16 they may overflow) and its
+// digits, because an error of theirs is one of the output before it is rounded. bf16 weights: the sum of three bf16 numbers,
+// 3 x 8 bits, which leaves 2^-24. fp16 weights: they are tf32 numbers as they stand, and the hidden value is the
+// sum of two of those, which leaves 2^-22. (Two bf16 terms for both, 2^-16, rounded two to three times as many outputs to a
+// neighbour of the plain form's value. For 64 tokens x 4 of 32 experts, 4096 x 1792, they took 291 us instead of 316 in bf16 and 322 instead of
+// 350 in fp16; for 16 tokens in fp16 157 both.)
 template <typename T>
-struct ActRow {
-  Vec<__nv_bfloat16, 8> hi, lo;
+struct ActRow;
+template <>
+struct ActRow<__nv_bfloat16> {
+  Vec<__nv_bfloat16, 8> v[3];
+};
+template <>
+struct ActRow<__half> {
+  Vec<float, 4> hi[2], lo[2];
 };
 template <>
 struct ActRow<float> {
@@ -310,54 +321,66 @@ struct ActRow<float> {
 };
 __device__ __forceinline__ void mul_act(float (&acc)[4], const ActRow<__nv_bfloat16>& a, const ActRow<__nv_bfloat16>& b,
                                         const Vec<__nv_bfloat16, 8>& w) {
-  mul_chunk<__nv_bfloat16>(acc, a.lo, b.lo, w);
-  mul_chunk<__nv_bfloat16>(acc, a.hi, b.hi, w);
+#pragma unroll
+  for (int i = 2; i >= 0; --i) mul_chunk<__nv_bfloat16>(acc, a.v[i], b.v[i], w);
 }
-// An fp16 number is the sum of two bf16 ones exactly: its 8 leading bits and the 3 below them. Of the four products the
-// smallest, lo x lo, is at most 2^-15 of the whole and left out.
 __device__ __forceinline__ void mul_act(float (&acc)[4], const ActRow<__half>& a, const ActRow<__half>& b,
                                         const Vec<__half, 8>& w) {
-  Vec<__nv_bfloat16, 8> hi, lo;
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w.v[i]));
-    const uint32_t x = __float_as_uint(f.x), y = __float_as_uint(f.y);
-    // (below 256 in size; the minimum takes the NaN that an infinite weight leaves here to a number)
-    const float rx = fminf(f.x - __uint_as_float(x & 0xffff0000u), 256.0f);
-    const float ry = fminf(f.y - __uint_as_float(y & 0xffff0000u), 256.0f);
-    *reinterpret_cast<uint32_t*>(&hi.v[i]) = __byte_perm(x, y, 0x7632);
-    *reinterpret_cast<uint32_t*>(&lo.v[i]) = __byte_perm(__float_as_uint(rx), __float_as_uint(ry), 0x7632);
+    const uint32_t w0 = __float_as_uint(f.x), w1 = __float_as_uint(f.y);
+    const int h = i / 4, j = i % 4;
+    mma_tf32(acc, __float_as_uint(a.lo[h].v[j]), __float_as_uint(b.lo[h].v[j]), __float_as_uint(a.lo[h].v[j + 1]),
+             __float_as_uint(b.lo[h].v[j + 1]), w0, w1);
+    mma_tf32(acc, __float_as_uint(a.hi[h].v[j]), __float_as_uint(b.hi[h].v[j]), __float_as_uint(a.hi[h].v[j + 1]),
+             __float_as_uint(b.hi[h].v[j + 1]), w0, w1);
   }
-  mul_chunk<__nv_bfloat16>(acc, a.lo, b.lo, hi);
-  mul_chunk<__nv_bfloat16>(acc, a.hi, b.hi, lo);
-  mul_chunk<__nv_bfloat16>(acc, a.hi, b.hi, hi);
 }
 __device__ __forceinline__ void mul_act(float (&acc)[4], const ActRow<float>& a, const ActRow<float>& b,
                                         const Vec<float, 4>& w) {
   mul_chunk(acc, a.v, b.v, w);
 }
+// `terms`: elements between the terms of a value
 template <typename T, bool WHOLE>
-__device__ __forceinline__ ActRow<T> load_act(const char* row, long long second, int k, int Fp) {
+__device__ __forceinline__ ActRow<T> load_act(const char* row, long long terms, int k, int Fp) {
   ActRow<T> r;
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (Elem<T>::kDtype == NSB_BF16) {
     const __nv_bfloat16* at = reinterpret_cast<const __nv_bfloat16*>(row);
-    r.hi = load_chunk<__nv_bfloat16, true, false, WHOLE>(at, k, Fp);
-    r.lo = load_chunk<__nv_bfloat16, true, false, WHOLE>(at + second, k, Fp);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) r.v[i] = load_chunk<__nv_bfloat16, true, false, WHOLE>(at + i * terms, k, Fp);
+  } else if constexpr (Elem<T>::kDtype == NSB_F16) {
+    const float* at = reinterpret_cast<const float*>(row);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r.hi[i] = load_chunk<float, true, false, WHOLE>(at, k + 4 * i, Fp);
+      r.lo[i] = load_chunk<float, true, false, WHOLE>(at + terms, k + 4 * i, Fp);
+    }
   } else {
     r.v = load_chunk<float, true, false, WHOLE>(reinterpret_cast<const float*>(row), k, Fp);
   }
   return r;
 }
 template <typename T>
+constexpr int kActBytes = Elem<T>::kDtype == NSB_BF16 ? 2 : 4;  // of a term
+template <typename T>
 __device__ __forceinline__ void store_act(void* act, long long slots, int slot, int Fp, int f, float v) {
-  if constexpr (sizeof(T) == 2) {
-    __nv_bfloat16* at = static_cast<__nv_bfloat16*>(act) + (long long)slot * Fp + f;
-    const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-    const float r = v - __bfloat162float(hi);
-    at[0] = hi;
-    at[slots * Fp] = __float2bfloat16_rn(isfinite(r) ? r : 0.0f);
+  const long long at = (long long)slot * Fp + f, terms = slots * Fp;
+  if constexpr (Elem<T>::kDtype == NSB_BF16) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const __nv_bfloat16 q = __float2bfloat16_rn(v);
+      static_cast<__nv_bfloat16*>(act)[at + i * terms] = q;
+      v -= __bfloat162float(q);
+      v = isfinite(v) ? v : 0.0f;
+    }
+  } else if constexpr (Elem<T>::kDtype == NSB_F16) {
+    uint32_t hi, lo;
+    split_tf32(v, hi, lo);
+    static_cast<uint32_t*>(act)[at] = hi;
+    static_cast<uint32_t*>(act)[at + terms] = lo;
   } else {
-    static_cast<float*>(act)[(long long)slot * Fp + f] = v;
+    static_cast<float*>(act)[at] = v;
   }
 }
 
@@ -521,21 +544,21 @@ __device__ __forceinline__ void down_unit(const MoeParams& p, int e, int first, 
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const T* w = static_cast<const T*>(p.w_out) + (long long)e * p.D * p.F;
   const char* rows[MT][2];
-  const long long second = (long long)p.N * p.K * p.Fp;
+  const long long terms = (long long)p.N * p.K * p.Fp;
   auto prepare = [&] {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         rows[m][h] = static_cast<const char*>(p.act) +
-                     (long long)p.slots[first + min(m * 16 + h * 8 + g, n - 1)] * p.Fp * (sizeof(T) == 2 ? 2 : 4);
+                     (long long)p.slots[first + min(m * 16 + h * 8 + g, n - 1)] * p.Fp * kActBytes<T>;
   };
   float acc[MT * 8];
 #pragma unroll
   for (int i = 0; i < MT * 8; ++i) acc[i] = 0.0f;
   weight_products<T, VEC, MT, kDownSteps>(
       acc, w + (long long)min(d0 + g, p.D - 1) * p.F, w + (long long)min(d0 + 8 + g, p.D - 1) * p.F, p.F, wk, WK, (n + 15) / 16, prepare,
-      [&](auto whole, int m, int h, int k) { return load_act<T, decltype(whole)::value>(rows[m][h], second, k, p.Fp); },
+      [&](auto whole, int m, int h, int k) { return load_act<T, decltype(whole)::value>(rows[m][h], terms, k, p.Fp); },
       [](float (&c)[4], const auto& a, const auto& b, const auto& q) { mul_act(c, a, b, q); });
   add_up<MT * 8>(acc, buf, wk, WK);
   if (wk != 0) return;
@@ -548,7 +571,7 @@ __device__ __forceinline__ void down_unit(const MoeParams& p, int e, int first, 
     }
 }
 template <typename T, bool VEC, int MT>
-__global__ void __launch_bounds__(kThreads, 5) moe_down_kernel(const MoeParams p, int WK) {
+__global__ void __launch_bounds__(kThreads, kDownCtas<T>) moe_down_kernel(const MoeParams p, int WK) {
   __shared__ float buf[MT * 8 * kThreads];
   __shared__ bool s_last;
   const int warp = threadIdx.x >> 5, per_cta = kWarps / WK;
@@ -618,7 +641,7 @@ Layout layout(long long N, long long E, long long K, long long D, long long F) {
   l.slots = l.entries + up16(12 * std::min(E, S));
   l.done = l.slots + up16(4 * S);
   l.act = l.done + up16(4 * ((D + 15) / 16));
-  l.part = l.act + 4 * S * Fp;
+  l.part = l.act + 8 * S * Fp;  // (fp16's; the others take less)
   l.bytes = l.part + 4 * S * D;
   return l;
 }

@@ -234,6 +234,24 @@ def test_no_gradients():
         mk.moe_few_tokens(x, wr, wi, wo, 2)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [1, 3, 40])
+def test_hidden_values_keep_their_digits(N, dtype):
+    """Hidden values that are whole numbers of 23 bits, and outputs that are small differences of two of them: everything on the
+    way is exact in fp32 (silu(g) = g where exp(-g) is below 2^-24, p = 1), and so is the output in its type."""
+    D, F = 16, 32
+    r = torch.arange(1, 17, device=DEV)
+    g = 2890 - 3 * r                                # h = g (g - 1 - r) < 2^23, beside it (g - 1) (g - r) = h + r
+    gate, up = torch.cat([g, g - 1]), torch.cat([g - 1 - r, g - r])
+    assert int((gate * up).max()) < 2 ** 23 and int((gate * up).min()) > 2 ** 22
+    bits = 2 ** torch.arange(D, device=DEV)
+    w_in = torch.cat([gate, up])[:, None].bitwise_and(bits).to(dtype)[None]
+    w_out = torch.cat([-torch.eye(16, device=DEV), torch.eye(16, device=DEV)], 1).to(dtype)[None]
+    x = torch.ones(N, D, device=DEV, dtype=dtype)
+    out = mk.moe_few_tokens(x, torch.zeros(1, D, device=DEV, dtype=dtype), w_in, w_out, 1)
+    assert torch.equal(out, r.to(dtype).expand(N, D))
+
+
 def test_long_sums_of_one_sign():
     """fp32, 32768 positive products a sum: rounding toward zero would lose some 1e-4 of each. Four warps share a row, so a warp
     adds 32768 / 16 / 4 = 512 chunks, each to the nearest: 512 / 2 half units in the last place (the partial sum is half of

@@ -638,10 +638,11 @@ __global__ void __launch_bounds__(kThreads, 3) gated_bwd_kernel(const GatedParam
         gate<V>(in.get(0, s), bias, f[s], m[s]);
         mine.H = fma<V>(f[s], mine.H, mul<V>(m[s], in.get(1, s)));
         mine.P = mul<V>(mine.P, f[s]);
-        // a state does not pass a sequence's border in either direction: one product serves both
-        if constexpr (kSpecial)
-          if (((rows.first | rows.last | ~rows.in) >> s) & 1u) mine.P = all<V>(kCut);
       }
+      // A state does not pass a sequence's border in either direction: one product serves both. The cut is made behind the
+      // products, which a NaN on either side of the border would undo.
+      if constexpr (kSpecial)
+        if ((rows.first | rows.last | ~rows.in) & ((1u << S) - 1u)) mine.P = all<V>(kCut);
 #pragma unroll
       for (int s = S - 1; s >= 0; --s) {
         if constexpr (kSpecial)

@@ -394,3 +394,22 @@ def test_second_derivatives_are_refused():
     with pytest.raises(nsb.NSBError, match="second derivatives"):
         torch.autograd.grad(y.sum(), x, create_graph=True)
     torch.autograd.grad(y.sum(), x)
+
+
+# one chunk; several that pass maps; several whose columns fill the GPU, so that states pass one by one
+@pytest.mark.parametrize("dtype,rows,D", [(torch.float32, 64, 8), (torch.bfloat16, 64, 64), (torch.float32, 1500, 40),
+                                          (torch.bfloat16, 1500, 66), (torch.float32, 200, 14300)])
+def test_a_nan_gate_does_not_reach_the_sequence_before(dtype, rows, D):
+    """Gradients of a packed batch: a NaN gate some rows behind a border, and a run without it."""
+    for border, behind in ((20, 2), (16, 5), (23, 1), (rows - 30, 3), (rows // 2 + 3, 4)):
+        v = make((rows, D), dtype, 67 + border, seqs=3)
+        cu = torch.tensor([0, border, rows - 9, rows], device=DEV)
+        clean = run(v, cu)
+        v["raw"][border + behind] = float("nan")
+        got = run(v, cu)
+        for n in ("y", "d_raw", "d_x"):
+            assert torch.equal(got[n][:border], clean[n][:border]), (n, border)
+            assert torch.equal(got[n][rows - 9:], clean[n][rows - 9:]), (n, border)
+        for n in ("h_last", "d_h0"):
+            assert torch.equal(got[n][::2], clean[n][::2]) and torch.isnan(got[n][1]).all(), (n, border)
+        assert torch.isnan(got["d_x"][border:border + behind]).all()

@@ -62,11 +62,12 @@ struct GatedParams {
 };
 
 // f = sigmoid(a + b) and m = sigmoid(-(a + b)) from e = exp(-(a + b)): f = 1 / (1 + e), m = e f, neither of them
-// a difference, so both keep their digits however small they are. The exponent is capped where f is 2^-126
-// (e f must not become inf * 0); min.NaN lets a NaN through. `b2` = -b log2(e).
+// a difference, so both keep their digits however small they are. a + b comes first: of two large numbers that nearly
+// cancel, scaled by log2(e) one by one, the roundings would be left. The exponent is capped where f is 2^-126
+// (e f must not become inf * 0); min.NaN lets a NaN through.
 template <int V>
-__device__ __forceinline__ void gate(const Cols<V>& a, const Cols<V>& b2, Cols<V>& f, Cols<V>& m) {
-  Cols<V> q = fma<V>(a, all<V>(-kLog2e), b2), e;
+__device__ __forceinline__ void gate(const Cols<V>& a, const Cols<V>& b, Cols<V>& f, Cols<V>& m) {
+  Cols<V> q = mul<V>(add<V>(a, b), all<V>(-kLog2e)), e;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(q[v]) : "f"(q[v]));  // 126
@@ -77,7 +78,6 @@ __device__ __forceinline__ void gate(const Cols<V>& a, const Cols<V>& b2, Cols<V
   for (int v = 0; v < V; ++v) f[v] = rcp(q[v]);
   m = mul<V>(e, f);
 }
-__device__ __forceinline__ float gate_bias(float b) { return b * -kLog2e; }
 
 __device__ __forceinline__ uint32_t publishable(float v) {
   const uint32_t b = __float_as_uint(v);
@@ -498,7 +498,6 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const GatedParam
     const bool plain = rows.plain(S);
     const Stage<T, V, S> in = stage(parity);
     if (ahead) copies_wait_but_last(); else copies_wait();
-    bias = mul<V>(bias, all<V>(-kLog2e));
 
     Cols<V> f[S], u[S];
     MapV<V> mine = {all<V>(1.0f), all<V>(0.0f)};
@@ -625,7 +624,6 @@ __global__ void __launch_bounds__(kThreads, 3) gated_bwd_kernel(const GatedParam
     const bool plain = rows.plain(S);
     const Stage<T, V, S> in = stage(parity);
     if (ahead) copies_wait_but_last(); else copies_wait();
-    bias = mul<V>(bias, all<V>(-kLog2e));
 
     Cols<V> f[S], m[S];
     TripleV<V> mine = {all<V>(1.0f), all<V>(0.0f), all<V>(0.0f)};
@@ -804,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, 3) gated_maps_kernel(const GatedPara
   const bool on = col < p.cols, whole = col - lane * V + 32 * V <= p.cols;  // (cols below 2^31 - 2^8)
   const T* raw = static_cast<const T*>(p.raw) + (on ? input_at(p, col, p.raw_st, p.raw_sb, 0) : 0);
   const T* x = static_cast<const T*>(p.x) + (on ? input_at(p, col, p.x_st, p.x_sb, 0) : 0);
-  const Cols<V> bias = mul<V>(load_bias<V>(p, col, on), all<V>(-kLog2e));
+  const Cols<V> bias = load_bias<V>(p, col, on);
   MapV<V> m = {all<V>(1.0f), all<V>(0.0f)};
   const ChunkRows kinds = chunk_rows<PACKED>(p, chunk * kCkptRows, lane);
   for (int i = 0; i < kCkptRows / S; ++i) {
@@ -908,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 3) gated_apply_kernel(const GatedPar
   const T* raw = static_cast<const T*>(p.raw) + (on ? input_at(p, col, p.raw_st, p.raw_sb, 0) : 0);
   const T* x = static_cast<const T*>(p.x) + (on ? input_at(p, col, p.x_st, p.x_sb, 0) : 0);
   T* y = static_cast<T*>(p.y) + col;
-  const Cols<V> bias = mul<V>(load_bias<V>(p, col, on), all<V>(-kLog2e));
+  const Cols<V> bias = load_bias<V>(p, col, on);
   Cols<V> h;
   const ChunkRows kinds = chunk_rows<PACKED>(p, chunk * kCkptRows, lane);
   for (int i = 0; i < kCkptRows / S; ++i) {
@@ -996,7 +994,7 @@ __global__ void __launch_bounds__(256) gated_step_kernel(const T* __restrict__ r
     Cols<V> c, f, m, hv;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      c[v] = bias ? gate_bias(bias[d + v]) : 0.0f;
+      c[v] = bias ? bias[d + v] : 0.0f;
       hv[v] = vh.v[v];
     }
     gate<V>(widen<T, V>(vr), c, f, m);

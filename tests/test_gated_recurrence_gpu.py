@@ -413,3 +413,27 @@ def test_a_nan_gate_does_not_reach_the_sequence_before(dtype, rows, D):
         for n in ("h_last", "d_h0"):
             assert torch.equal(got[n][::2], clean[n][::2]) and torch.isnan(got[n][1]).all(), (n, border)
         assert torch.isnan(got["d_x"][border:border + behind]).all()
+
+
+def test_gates_that_nearly_cancel():
+    """raw + bias is a small exact difference of two large numbers: the gate goes by it, not by their sizes."""
+    T, B, D = 300, 2, 40
+    v = make((T, B, D), torch.float32, 71)
+    a = torch.randint(-2048, 2049, (T, B, D), device=DEV) * 2.0 ** -9
+    # (biases that a power of two does not divide much further: log2(e) times them is not exact)
+    v["bias"] = (12345.0 + torch.arange(D, device=DEV) * 7.125) * torch.where(torch.arange(D, device=DEV) % 2 == 0, 1.0, -1.0)
+    v["raw"] = a - v["bias"]
+    assert torch.equal(v["raw"].double() + v["bias"].double(), a.double())
+    want = reference(v["raw"], v["x"], v["h0"], v["bias"], None, v["dy"], v["dh"])
+    compare(run(v), want, torch.float32)
+    h = v["h0"].clone()
+    for t in range(6):
+        y = gr.gated_linear_recurrence_step(v["raw"][t], v["x"][t], h, v["bias"])
+        close(y, tuple(w[t] for w in want["y"]), torch.float32, "step")
+    T = 24000  # long enough for three launches
+    v = make((T, 1, 700), torch.float32, 73)
+    v["bias"] = torch.full((700,), 12345.0, device=DEV)
+    v["raw"] = torch.randint(-2048, 2049, (T, 1, 700), device=DEV) * 2.0 ** -9 - 12345.0
+    with torch.no_grad():
+        y, _ = gr.gated_linear_recurrence(v["raw"], v["x"], v["h0"], v["bias"])
+    close(y, reference(v["raw"], v["x"], v["h0"], v["bias"])["y"], torch.float32, "y")

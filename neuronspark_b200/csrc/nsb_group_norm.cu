@@ -245,10 +245,11 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rows_bwd_kernel(const NormPa
 struct Moments {
   float n, mean, m2;
 };
-// Both parts' values as one (Chan, Golub and LeVeque 1979)
+// Both parts' values as one (Chan, Golub and LeVeque 1979). The weight comes first: beside an empty part d is a whole mean,
+// whose square may overflow, and counts nothing.
 __device__ __forceinline__ Moments join(Moments a, Moments b) {
   const float n = a.n + b.n, d = b.mean - a.mean, f = n > 0.0f ? __fdividef(b.n, n) : 0.0f;
-  return {n, fmaf(d, f, a.mean), a.m2 + b.m2 + d * d * a.n * f};
+  return {n, fmaf(d, f, a.mean), fmaf(a.n * f * d, d, a.m2 + b.m2)};
 }
 __device__ __forceinline__ Moments warp_join(Moments m) {
 #pragma unroll

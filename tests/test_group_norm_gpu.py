@@ -294,3 +294,15 @@ def test_second_derivatives_are_refused():
     with pytest.raises(nsb.NSBError, match="second derivatives"):
         torch.autograd.grad(y.sum(), x, create_graph=True)
     torch.autograd.grad(y.sum(), x)
+
+
+@pytest.mark.parametrize("shape,G", [((7, 96), 3), ((2, 70, 96), 3), ((1, 1000, 40), 1), ((3, 600), 1), ((2, 33, 520), 2)], ids=str)
+def test_means_whose_square_overflows(shape, G):
+    """A finite variance about a mean of 1e20, in both layouts."""
+    _, w, b, dy = make(shape, torch.float32, 31)
+    g = torch.Generator(device=DEV).manual_seed(37)
+    x = 1e20 * (1 + 1e-4 * torch.randn(shape, generator=g, device=DEV))
+    assert torch.isinf(x.mean() ** 2) and torch.isfinite((x - x.mean()).square().sum())
+    want = reference(x, G, w, b, dy)
+    for n, t in run(x, G, w, b, dy).items():
+        close(t, want[n], n)

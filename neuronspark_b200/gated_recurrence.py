@@ -136,7 +136,7 @@ def gated_linear_recurrence(raw_gate: torch.Tensor, x: torch.Tensor, h0: torch.T
 def gated_linear_recurrence_step(raw_gate: torch.Tensor, x: torch.Tensor, h: torch.Tensor,
                                  bias: torch.Tensor | None = None) -> torch.Tensor:
     """One token for each of B running sequences: ``raw_gate``, ``x`` [B, D]; the fp32 state ``h`` [B, D] is
-    updated in place and returned rounded to ``x``'s type. No gradients."""
+    updated in place and returned rounded to ``x``'s type. No gradients; to autograd it is a change in place of ``h``."""
     if x.dim() != 2 or raw_gate.shape != x.shape or h.shape != x.shape:
         raise NSBError("gated_linear_recurrence_step expects raw_gate, x and h of one shape [B, D]")
     if h.dtype != torch.float32 or not h.is_contiguous():
@@ -152,4 +152,6 @@ def gated_linear_recurrence_step(raw_gate: torch.Tensor, x: torch.Tensor, h: tor
     at = _lib.address
     _lib.launch(dev, "nsb_gated_recurrence_step", at(a), a.stride(0), at(v), v.stride(0), at(b), at(h), at(y), x.shape[0],
                 x.shape[1], code)
+    if not h.is_inference():  # a graph that has saved h must not take the new state for the old one
+        torch.autograd.graph.increment_version(h)
     return y if dt == x.dtype else _cast(y, x.dtype)

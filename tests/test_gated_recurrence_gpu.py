@@ -437,3 +437,21 @@ def test_gates_that_nearly_cancel():
     with torch.no_grad():
         y, _ = gr.gated_linear_recurrence(v["raw"], v["x"], v["h0"], v["bias"])
     close(y, reference(v["raw"], v["x"], v["h0"], v["bias"])["y"], torch.float32, "y")
+
+
+def test_a_step_counts_as_a_change_of_the_state():
+    """A state that a graph has saved and that is stepped afterwards: the backward pass is refused, as after any change in place."""
+    v = make((5, 3, 16), torch.float32, 79)
+    h = v["h0"].clone().requires_grad_()
+    raw = v["raw"].clone().requires_grad_()
+    y, _ = gr.gated_linear_recurrence(raw, v["x"], h)
+    before = h._version
+    with torch.no_grad():
+        gr.gated_linear_recurrence_step(v["raw"][0], v["x"][0], h)
+    assert h._version > before
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y.sum(), raw)
+    with torch.inference_mode():
+        state = v["h0"].clone()  # has no version to count
+        out = gr.gated_linear_recurrence_step(v["raw"][0], v["x"][0], state)
+        assert torch.equal(out, state)

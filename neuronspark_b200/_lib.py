@@ -188,6 +188,12 @@ def launch(dev: torch.device, name: str, *args) -> None:
         check(status, name)
 
 
+def wants_gradients(*tensors) -> bool:
+    """Whether a backward pass through a call with these tensors can come. (In an autograd function's forward
+    ``ctx.needs_input_grad`` says that they require gradients under ``no_grad`` as well.)"""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def require_cuda(*tensors) -> torch.device:
     dev = None
     for t in tensors:

@@ -56,7 +56,7 @@ class GatedLinearRecurrence(torch.autograd.Function):
     """``(y, h_last)``; gradients for raw_gate, x, h0 and bias, through both outputs."""
 
     @staticmethod
-    def forward(ctx, raw_gate, x, h0, bias, cu):
+    def forward(ctx, raw_gate, x, h0, bias, cu, needs_grad):
         dt = x.dtype if raw_gate.dtype == x.dtype else _common_stream_dtype(raw_gate, x)
         code = _lib.dtype_code(dt)
         a, v = _strided(raw_gate, dt), _strided(x, dt)
@@ -68,7 +68,6 @@ class GatedLinearRecurrence(torch.autograd.Function):
         L, at = _lib.lib(), _lib.address
         y = torch.empty(x.shape, dtype=dt, device=dev)
         h_last = torch.empty(state, dtype=torch.float32, device=dev)
-        needs_grad = any(ctx.needs_input_grad)
         chunks, words = L.nsb_gated_chunks(T), L.nsb_gated_scratch_words(T, B * D)
         ckpt = torch.empty(chunks * B * D, dtype=torch.float32, device=dev) if needs_grad and chunks > 1 else None
         scratch = torch.empty(words, dtype=torch.int32, device=dev) if words else None
@@ -91,7 +90,7 @@ class GatedLinearRecurrence(torch.autograd.Function):
         dev, dt, L, at = a.device, a.dtype, _lib.lib(), _lib.address
         dy = torch.zeros(v.shape, dtype=dt, device=dev) if dy is None else _lib.convert(dy, dt)
         dh = None if dh_last is None else dh_last.contiguous()
-        want_a, want_x, want_h, want_b, _ = ctx.needs_input_grad
+        want_a, want_x, want_h, want_b = ctx.needs_input_grad[:4]
         d_raw = torch.empty(a.shape, dtype=dt, device=dev) if want_a else None
         d_x = torch.empty(v.shape, dtype=dt, device=dev) if want_x else None
         d_h0 = torch.empty(ctx.state, dtype=torch.float32, device=dev) if want_h and h0 is not None else None
@@ -104,7 +103,7 @@ class GatedLinearRecurrence(torch.autograd.Function):
                     cu.shape[0] - 1 if cu is not None else 0, at(ckpt), at(dy), at(dh), at(d_raw), at(d_x), at(d_bias),
                     at(d_h0), part, at(scratch), T, B, D, _lib.dtype_code(dt))
         return (*(g if g is None or g.dtype == t else _cast(g, t) for g, t in zip((d_raw, d_x, d_h0, d_bias), ctx.in_dtypes)),
-                None)
+                None, None)
 
 
 def gated_linear_recurrence(raw_gate: torch.Tensor, x: torch.Tensor, h0: torch.Tensor | None = None,
@@ -130,7 +129,7 @@ def gated_linear_recurrence(raw_gate: torch.Tensor, x: torch.Tensor, h0: torch.T
         if cu_seqlens.dtype not in (torch.int32, torch.int64):
             raise NSBError(f"cu_seqlens has type {cu_seqlens.dtype}; expected int32 or int64")
         cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
-    return GatedLinearRecurrence.apply(raw_gate, x, h0, bias, cu_seqlens)
+    return GatedLinearRecurrence.apply(raw_gate, x, h0, bias, cu_seqlens, _lib.wants_gradients(raw_gate, x, h0, bias))
 
 
 def gated_linear_recurrence_step(raw_gate: torch.Tensor, x: torch.Tensor, h: torch.Tensor,

@@ -455,3 +455,22 @@ def test_a_step_counts_as_a_change_of_the_state():
         state = v["h0"].clone()  # has no version to count
         out = gr.gated_linear_recurrence_step(v["raw"][0], v["x"][0], state)
         assert torch.equal(out, state)
+
+
+def test_nothing_is_kept_for_a_backward_that_cannot_come():
+    """A bias that is a parameter, as a module has it, costs no saved states without gradients."""
+    v = make((400, 2, 64), torch.bfloat16, 83)
+    cu = torch.tensor([0, 150, 400], device=DEV)
+
+    def allocations(bias):
+        def count():
+            return torch.cuda.memory_stats(DEV)["allocation.all.allocated"]
+        before = count()
+        gr.gated_linear_recurrence(v["raw"], v["x"], v["h0"], bias)
+        gr.gated_linear_recurrence(v["raw"][:, 0].contiguous(), v["x"][:, 0].contiguous(), v["h0"], bias, cu)
+        return count() - before
+    parameter = torch.nn.Parameter(v["bias"].clone())
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            assert allocations(parameter) == allocations(v["bias"])
+    assert allocations(parameter) > allocations(v["bias"])  # (with gradients there are some to keep)

@@ -29,7 +29,7 @@ def _param(t):
 
 class GroupNormAct(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, num_groups, eps, act):
+    def forward(ctx, x, weight, bias, num_groups, eps, act, needs_grad):
         x_c, w, b = x.contiguous(), _param(weight), _param(bias)
         dev = _lib.require_cuda(x_c, w, b)
         shape = x.shape
@@ -37,7 +37,6 @@ class GroupNormAct(torch.autograd.Function):
         L = x_c.numel() // (N * C) if N * C else 0
         lib, at = _lib.lib(), _lib.address
         y = torch.empty(shape, dtype=x.dtype, device=dev)
-        needs_grad = any(ctx.needs_input_grad)
         stats = torch.empty(2 * N * num_groups, dtype=torch.float32, device=dev) if needs_grad else None
         words = lib.nsb_group_norm_scratch_floats(N, L, C, num_groups, 0)
         scratch = torch.empty(words, dtype=torch.float32, device=dev) if words else None
@@ -69,7 +68,8 @@ class GroupNormAct(torch.autograd.Function):
         rstd = mean + 4 * N * G if mean else None
         _lib.launch(dev, "nsb_group_norm_bwd", at(dy), at(x), at(w), at(b), mean, rstd, at(dx), at(dw), at(db), at(scratch),
                     N, L, C, G, act, _lib.dtype_code(x.dtype))
-        return (dx, *(g if g is None or g.dtype == t else g.to(t) for g, t in zip((dw, db), ctx.in_dtypes)), None, None, None)
+        return (dx, *(g if g is None or g.dtype == t else g.to(t) for g, t in zip((dw, db), ctx.in_dtypes)), None, None, None,
+                None)
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -87,7 +87,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     if activation not in _ACTIVATIONS:
         raise NSBError(f"unknown activation {activation!r}; expected 'silu' or None")
     _lib.dtype_code(x.dtype)
-    return GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps), _ACTIVATIONS[activation])
+    return GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps), _ACTIVATIONS[activation],
+                              _lib.wants_gradients(x, weight, bias))
 
 
 class GroupNorm(nn.Module):

@@ -306,3 +306,21 @@ def test_means_whose_square_overflows(shape, G):
     want = reference(x, G, w, b, dy)
     for n, t in run(x, G, w, b, dy).items():
         close(t, want[n], n)
+
+
+def test_nothing_is_kept_for_a_backward_that_cannot_come():
+    """A module's parameters cost no saved statistics without gradients."""
+    norm = gn.GroupNorm(6, 96).to(DEV)
+    w, b = norm.weight.detach().clone(), norm.bias.detach().clone()
+
+    def allocations(call):
+        before = torch.cuda.memory_stats(DEV)["allocation.all.allocated"]
+        call()
+        return torch.cuda.memory_stats(DEV)["allocation.all.allocated"] - before
+    for shape in ((50, 96), (2, 70, 96)):
+        x = torch.randn(shape, device=DEV)
+        for mode in (torch.no_grad, torch.inference_mode):
+            with mode():
+                assert allocations(lambda: norm(x)) == allocations(lambda: gn.group_norm_act(x, 6, w, b))
+                assert torch.equal(norm(x), gn.group_norm_act(x, 6, w, b))
+        assert allocations(lambda: norm(x)) > allocations(lambda: gn.group_norm_act(x, 6, w, b))

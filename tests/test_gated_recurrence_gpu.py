@@ -474,3 +474,62 @@ def test_nothing_is_kept_for_a_backward_that_cannot_come():
         with mode():
             assert allocations(parameter) == allocations(v["bias"])
     assert allocations(parameter) > allocations(v["bias"])  # (with gradients there are some to keep)
+
+
+EMPTY = {"middle": lambda n: [0, 5] + [5] * n + [9, 200], "end": lambda n: [0, 100, 200] + [200] * n, "start": lambda n: [0] * (n + 1) + [200],
+         "twice": lambda n: [0, 3] + [3] * n + [11] * n + [14, 14, 70, 200], "before the last row": lambda n: [0, 199] + [199] * n + [200]}
+
+
+@pytest.mark.parametrize("n", [29, 30, 31, 32, 33, 70])
+@pytest.mark.parametrize("where", EMPTY)
+def test_many_empty_sequences_in_a_row(where, n):
+    """Rows of one warp that dozens of sequences end in."""
+    cu = EMPTY[where](n)
+    for dtype, D in ((torch.float32, 5), (torch.bfloat16, 64)):
+        v = make((200, D), dtype, 89 + n, seqs=len(cu) - 1)
+        compare(run(v, torch.tensor(cu, device=DEV)), reference(v["raw"], v["x"], v["h0"], v["bias"], cu, v["dy"], v["dh"]), dtype)
+
+
+@pytest.mark.parametrize("seqs", [1025, 5000])
+def test_thousands_of_sequences(seqs):
+    """Most of them empty: the search goes over more than 1024."""
+    g = torch.Generator().manual_seed(seqs)
+    cu = [0] + sorted(torch.randint(0, 391, (seqs - 1,), generator=g).tolist()) + [390]
+    v = make((400, 34), torch.bfloat16, 97, seqs=seqs)
+    compare(run(v, torch.tensor(cu, device=DEV)), reference(v["raw"], v["x"], v["h0"], v["bias"], cu, v["dy"], v["dh"]), torch.bfloat16)
+
+
+@pytest.mark.parametrize("seqs", [7, 2000])
+def test_gradients_of_a_long_packed_forward(seqs):
+    """45 MB of inputs, so that the forward takes three launches and the backward starts from the states of the second."""
+    rows, D = 14001, 800
+    g = torch.Generator().manual_seed(seqs)
+    cu = [0] + sorted(torch.randint(0, rows - 20, (seqs - 1,), generator=g).tolist()) + [rows - 20]
+    v = make((rows, D), torch.bfloat16, 101, seqs=seqs)
+    compare(run(v, torch.tensor(cu, device=DEV)), reference(v["raw"], v["x"], v["h0"], v["bias"], cu, v["dy"], v["dh"]), torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype,T,D", [(torch.float32, 20000, 48), (torch.bfloat16, 9000, 130), (torch.bfloat16, 300, 28500)])
+def test_slow_gates(dtype, T, D):
+    """Gates around 0.995: states and their gradients live for hundreds of steps, over many chunks."""
+    v = make((T, 1, D), dtype, 103, spread=0.5)
+    v["raw"] = (v["raw"].float() + 4.3).to(dtype)
+    compare(run(v), reference(v["raw"], v["x"], v["h0"], v["bias"], None, v["dy"], v["dh"]), dtype)
+
+
+def test_captured_steps():
+    """One token's step in a graph: every replay goes on from the state that the last one left."""
+    v = make((6, 20, 96), torch.bfloat16, 107)
+    raw, x, h = v["raw"][0].clone(), v["x"][0].clone(), v["h0"].clone()
+    gr.gated_linear_recurrence_step(raw, x, h.clone(), v["bias"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = gr.gated_linear_recurrence_step(raw, x, h, v["bias"])
+    h.copy_(v["h0"])
+    eager = v["h0"].clone()
+    for t in range(6):
+        raw.copy_(v["raw"][t])
+        x.copy_(v["x"][t])
+        graph.replay()
+        want = gr.gated_linear_recurrence_step(v["raw"][t], v["x"][t], eager, v["bias"])
+        assert torch.equal(y, want) and torch.equal(h, eager)

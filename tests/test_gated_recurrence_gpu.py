@@ -533,3 +533,27 @@ def test_captured_steps():
         graph.replay()
         want = gr.gated_linear_recurrence_step(v["raw"][t], v["x"][t], eager, v["bias"])
         assert torch.equal(y, want) and torch.equal(h, eager)
+
+
+def test_gates_are_as_good_as_rounded():
+    """A state of one and an input of zero: y = f. An error of f counts 1 / (1 - f) times in a long run, so it has to be
+    little more than that of a rounding, 2^-25 for f in 1/2 .. 1. The exponential is off by 2 units in the last place and its argument
+    by 1.3 |a| 2^-24, together (4 + 1.3 |a|) 2^-24, of which f takes f (1 - f) parts; below 1/2 the residual 1 - f - e f has
+    a rounding of 2^-25, and f one of its own, 2^-24 of it."""
+    rows, D = 14001, 800
+    g = torch.Generator(device=DEV).manual_seed(109)
+    raw = 16 * torch.rand(rows, D, generator=g, device=DEV) - 6
+    a = raw.double()
+    f = torch.sigmoid(a)
+    bound = torch.where(f >= 0.5, torch.full_like(f, 2.0 ** -25), 1.5 * U * f) + f * (1 - f) * (4 + 1.3 * a.abs()) * U
+    ones, zeros = torch.ones(rows, D, device=DEV), torch.zeros(rows, D, device=DEV)
+    own = torch.arange(rows + 1, device=DEV)  # a sequence for each row
+    for what, y in (("step", gr.gated_linear_recurrence_step(raw, zeros, ones.clone())),
+                    ("three launches", gr.gated_linear_recurrence(raw, zeros, ones, None, own)[0]),
+                    ("one launch", gr.gated_linear_recurrence(raw[:3000], zeros[:3000], ones[:3000], None, own[:3001])[0]),
+                    ("time-major", gr.gated_linear_recurrence(raw[None], zeros[None], ones)[0][0])):
+        assert ((y.double() - f[:len(y)]).abs() <= bound[:len(y)]).all(), what
+    h0 = ones.clone().requires_grad_()
+    y, h = gr.gated_linear_recurrence(raw, zeros, h0, None, own)
+    d = torch.autograd.grad(y, h0, ones)[0]
+    assert ((d.double() - f).abs() <= bound).all(), "gradient"

@@ -704,8 +704,9 @@ int nsb_modulation_fwd(const void* raw_beta, const void* raw_alpha, const void* 
  * Packed sequences: B = 1 and cu_seqlens = seqs + 1 int32 in device memory; sequence s is
  * rows cu_seqlens[s] .. cu_seqlens[s+1]-1, it starts from h0[s] and leaves h_last[s]
  * ([seqs, D]). Lengths may be zero (h_last = h0). Rows outside of every sequence get y = 0.
- * The values must not decrease; whatever they are, nothing outside the T rows and the
- * `seqs` states is touched. cu_seqlens = NULL and seqs = 0: B sequences of T rows.
+ * The values must not decrease and lie in 0 .. T (a sequence whose last row is not among
+ * the T leaves its h_last and d_h0 unwritten); whatever they are, nothing outside the T rows
+ * and the `seqs` states is touched. An infinite state goes on as infinite or NaN. cu_seqlens = NULL and seqs = 0: B sequences of T rows.
  *
  * ckpt: NULL, or nsb_gated_chunks(T) * B * D floats for the backward.
  * scratch: nsb_gated_scratch_words(T, B*D) words that the call overwrites, 16-byte
@@ -768,7 +769,7 @@ int nsb_moe_few_tokens(const void* x, int64_t x_stride, const void* w_router, co
  * weight, bias [C] fp32 or NULL (ones, zeros). mean, rstd [N, G] fp32: both or neither,
  * written for the backward. Variance (over n, not n - 1) about the mean, fp32 sums.
  * scratch: nsb_group_norm_scratch_floats floats, needed where that is not 0; one buffer per
- * call in flight. The reference has no counterpart; its normaliser takes whole rows and
+ * call in flight (backward, where L > 1 or C/G > 256: 2*C floats per sample and more). The reference has no counterpart; its normaliser takes whole rows and
  * subtracts no mean (atomic_ops/lateral_inhibition.py:50-119).
  */
 int64_t nsb_group_norm_scratch_floats(int64_t N, int64_t L, int64_t C, int64_t G, int backward);

@@ -7,7 +7,7 @@
 //   G_t = dy_t + K_{t+1}     dx_t = (1 - f_t) G_t     draw_t = G_t (h_{t-1} - x_t) f_t (1 - f_t)
 //
 // Each step is an affine map of the state, h -> P h + H, and such maps compose associatively, so time is
-// cut into chunks that are worked on side by side. A tile is one chunk (at most 64 steps) of one block of columns:
+// cut into chunks that are worked on side by side. A tile is one chunk (at most 128 steps, 64 in the backward) of one block of columns:
 // every warp has S steps of 32 V columns in registers, finds their composed map, the CTA's warps exchange
 // their maps through shared memory, CTAs exchange theirs through global memory (below), and every warp then
 // runs its steps once more from its true starting state. Each input is read once and each output written
@@ -741,8 +741,9 @@ __global__ void __launch_bounds__(kThreads, 3) gated_bwd_kernel(const GatedParam
 // packed sequences the search for those of a tile's rows lies on that path. Three launches read the inputs twice
 // instead: the chunks' maps, their composition along time, then every chunk from its starting state. A warp has 64 steps
 // of 32 V columns to itself, one after the other, so nothing is kept, exchanged or waited for inside a launch. Blocks whose
-// rows and columns are all there load without conditions (32 + 38 us before, for 32768 x 768 bf16). Now 28 + 6 + 33 us, 3.6 and
-// 4.6 TB/s, at half an instruction per cycle and scheduler: bound by neither alone.
+// rows and columns are all there load without conditions (28 + 33 us where 32 + 38 were, for 32768 x 768 bf16, before the gate's
+// Newton step). Now 29 + 8 + 34 us, 3.5 and 4.4 TB/s, at half an instruction per cycle and scheduler and 28 % of the warps' places
+// taken (384 CTAs for 444 places): what is loaded is waited for with little else to do.
 
 // row_kinds of a whole chunk at once: the search for the sequences of its rows runs once, a row per lane and turn
 struct ChunkRows {
@@ -1069,11 +1070,17 @@ int start_kernel(const GatedParams& p, int ctas, int device, cudaStream_t st) {
 
 // Three launches read the inputs twice and cost some 25 us of their own, but in none does a chunk wait for another. They
 // are taken for packed sequences (whose search lies on the path of the hand-over) from 40 MB of inputs, else from 64 MB
-// and where there are few columns for the steps. Forward in us, three launches and one, inputs not in any cache: packed
-// 16384 x 768 bf16 53 and 61, 24000 x 768 53 and 79, 32768 x 768 61 and 105, 32768 x 6144 338 and 582, 20011 x 1001 fp16 70
-// and 145; not packed 16384 x 768 bf16 44 and 43, 32768 x 768 59 and 76, 65536 x 768 fp32 171 and 206, 20011 x 1001 fp16
-// 64 and 101, 16384 x 4096 bf16 130 and 137, 2048 x 49152 204 and 155, 512 x 393216 487 and 304. The backward's three
-// launches came out within 8% either way of its one, and were dropped.
+// and where there are few columns for the steps. Forward in us, three launches and one, inputs not in any cache:
+//   packed, three taken   bf16 13100 x 768 43 and 51, 16384 x 768 51 and 61, 24000 x 768 55 and 78, 32768 x 768 63 and 104,
+//     4096 x 6144 64 and 139, 32768 x 6144 352 and 590; fp16 20011 x 1001 71 and 146
+//   packed, one taken     bf16 8192 x 768 30 and 37, 12288 x 768 35 and 49: the slower side (with 24 sequences)
+//   else, three taken     bf16 24000 x 768 53 and 57, 32768 x 768 61 and 74, 65536 x 768 110 and 137; fp32 32768 x 768 90 and 109,
+//     65536 x 768 172 and 204; fp16 20011 x 1001 66 and 102; bf16 32768 x 2048 135 and 155
+//   else, one taken       bf16 12288 x 768 33 and 33, 16384 x 768 49 and 43, 8192 x 6144 106 and 102,
+//     2048 x 49152 210 and 158, 8192 x 49152 680 and 578, 512 x 393216 498 and 311, fp32 16384 x 6144 313 and 293, fp16 20001 x 8008
+//     297 and 297; the slower side by 1 to 5 %: bf16 16384 x 2048 82 and 84, 16384 x 4096 135 and 138, 16384 x 6144 188 and 190,
+//     32768 x 6144 346 and 364
+// The backward's three launches came out within 8% either way of its one, and were dropped.
 bool three_launches(long long T, long long cols, size_t es, bool packed) {
   const double bytes = 2.0 * (double)T * (double)cols * (double)es;
   return packed ? bytes >= 40e6 : bytes >= 64e6 && T / 16 >= cols;

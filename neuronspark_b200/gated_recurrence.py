@@ -116,7 +116,11 @@ def gated_linear_recurrence(raw_gate: torch.Tensor, x: torch.Tensor, h0: torch.T
     Packed sequences: ``raw_gate`` and ``x`` [rows, D] and ``cu_seqlens``, seqs + 1 integers on the device that do
     not decrease; sequence s is rows ``cu_seqlens[s]`` to ``cu_seqlens[s+1] - 1`` and has ``h0[s]`` and
     ``h_last[s]`` ([seqs, D]). A sequence may be empty; rows outside of all sequences get zero, in ``y`` and in
-    the gradients. The values of ``cu_seqlens`` are not looked at by the host.
+    the gradients. Nothing, NaN included, passes from one sequence to another. The values of ``cu_seqlens`` are not looked at
+    by the host; they have to lie in 0 .. rows (a sequence whose last row is not there leaves its ``h_last`` unwritten).
+
+    An infinite state goes on as infinite or NaN. There are no second derivatives: a backward pass with
+    ``create_graph=True`` is refused.
 
     Inputs must not be changed in place between forward and backward. The first call of a process must not be
     made inside a CUDA stream capture (nor may that of the scans; it sets up the library's error word)."""

@@ -75,7 +75,12 @@ class GroupNormAct(torch.autograd.Function):
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                    eps: float = 1e-5, activation: str | None = "silu") -> torch.Tensor:
     """``x`` [N, ..., C] (float32, bfloat16 or float16), ``weight`` and ``bias`` [C] or None. ``activation`` is
-    "silu" or None. Returns a contiguous tensor of ``x``'s shape and type; gradients for x, weight and bias."""
+    "silu" or None. Returns a contiguous tensor of ``x``'s shape and type; gradients for x, weight and bias. There are no
+    second derivatives: a backward pass with ``create_graph=True`` is refused.
+
+    Made for groups of up to 256 channels where a sample has one position, and for samples of 64 positions and more
+    otherwise. Wider groups and shorter samples are right but slow (65536 x 768 in 2 groups takes longer than elementary torch
+    operations), and their backward pass takes 8 bytes of workspace per sample and channel."""
     if x.dim() < 2:
         raise NSBError("group_norm_act expects x of [N, ..., C]")
     C = x.shape[-1]
